@@ -95,6 +95,16 @@ PROTOTYPES = {
     "axhip_linear_f16_packed": (c_i, [c_vp, c_i, c_vp, c_vp, c_vp, c_i, c_i64, c_i64, c_i64, c_i, c_vp]),
     "axhip_embedding": (c_i, [c_vp, c_i, c_vp, c_vp, c_i, c_i64, c_i64, c_i64, c_vp]),
     "axhip_argmax": (c_i, [c_vp, c_vp, c_i, c_i64, c_i64, c_vp]),
+    "axhip_rotary_qk": (c_i, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_f, c_i, c_i, c_vp, c_vp, c_i, c_i64, c_i, c_i, c_i, c_vp]),
+    "axhip_rotary_inv_freq": (c_i, [c_i, C.c_double, c_i, C.c_double, c_i64, C.c_double, C.c_double, c_vp, c_vp]),
+    "axhip_rotary_append_paged": (c_i, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i, c_vp, c_vp, c_i, c_f, c_i, c_vp, c_i, c_vp,
+                                        c_f, c_i, c_i, c_i, c_i, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i, c_i, c_i, c_i, c_i, c_i,
+                                        c_i, c_i, c_vp]),
+    "axhip_chunk_attention_paged_workspace_bytes": (c_sz, [c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_i]),
+    "axhip_chunk_attention_paged": (c_i, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_sz, c_i, c_i, c_i, c_i, c_i, c_i,
+                                          c_i, c_i, c_i, c_i, c_vp]),
+    "axhip_logits_process": (c_i, [c_vp, c_i64, c_i, c_vp, c_i, c_i64, c_i64, c_i, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i,
+                                   c_vp, c_i64, c_vp, c_i64, c_i, c_i, c_vp]),
     "axhip_prefill_attention_tune": (None, [c_i]),
     "axhip_prefill_attention": (c_i, [c_vp, c_vp, c_vp, c_vp, c_vp, c_i, c_i, c_i, c_i, c_i, c_i, c_i, c_vp]),
     "axhip_gqa_decode_qkv": (c_i, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i, c_f, c_vp, c_vp, c_i, c_i, c_vp,

@@ -387,6 +387,81 @@ AXHIP_API int axhip_rope_with_cos_sin(const void *x, const float *cos_t, const f
                                       void *out, int dtype, int64_t rows, int64_t heads,
                                       int64_t dim, axhip_stream stream);
 
+/* Rotation of q and k by a table of frequencies: pairs in either layout, part of the head, tables scaled for long
+ * contexts.  Pair i < rotary_dim / 2 is (x_i, x_{i + rotary_dim/2}), or (x_{2i}, x_{2i+1}) when `interleaved`, and turns
+ * by the angle a = pos * inv_freq_i:  y0 = scale (x0 cos a - x1 sin a), y1 = scale (x1 cos a + x0 sin a); elements from
+ * rotary_dim on are copied.  The angle is formed in 64 bits (positions of any size and sign), the rest in fp32 with one
+ * rounding at the store.  Negated positions give the transpose, which is the gradient's map.
+ *   q [rows, q_heads, dim], k [rows, k_heads, dim], `dtype`; rows q_stride / k_stride elements apart, heads contiguous
+ *   pos device int64[rows]; inv_freq device fp32[rotary_dim / 2] (axhip_rotary_inv_freq); scale: on cosine and sine
+ *   q_out, k_out contiguous; each may be its input when that is contiguous
+ * q_heads or k_heads may be 0.  dim % 8 == 0, dim <= 512, rotary_dim even.  Interleaved pairs start on even elements:
+ * pointers and strides that would put one across a boundary of two elements return AXHIP_INVALID_ARGUMENT.
+ * The reference rotates whole heads in the half layout only (ops::cuda::Rope, src/ops/cuda/sequence.cu:84-101,318-342). */
+AXHIP_API int axhip_rotary_qk(const void *q, int64_t q_stride, const void *k, int64_t k_stride, const int64_t *pos,
+                              const float *inv_freq, float scale, int interleaved, int rotary_dim, void *q_out,
+                              void *k_out, int dtype, int64_t rows, int q_heads, int k_heads, int dim,
+                              axhip_stream stream);
+
+/* The table for axhip_rotary_qk, computed on the host into host memory (upload it once): f_i = theta^(-2 i / rotary_dim),
+ *   LINEAR  f_i / factor;   NTK  theta replaced by theta factor^(rotary_dim / (rotary_dim - 2));
+ *   YARN    f_i k + (f_i / factor)(1 - k), k = clamp((trained_len f_i / 2 pi - slow_turns) / (fast_turns - slow_turns), 0, 1):
+ *           pairs that turn at least fast_turns times over the trained context keep their frequency, pairs that turn
+ *           at most slow_turns times are divided.  *scale = 0.1 ln(factor) + 1 for factor > 1.
+ * theta > 0, factor > 0 (PLAIN ignores it), rotary_dim even and at most 512; trained_len, fast_turns and slow_turns are
+ * read for YARN only.  *scale (may be NULL) is 1 for the other kinds.  No reference counterpart. */
+#define AXHIP_ROTARY_PLAIN 0
+#define AXHIP_ROTARY_LINEAR 1
+#define AXHIP_ROTARY_NTK 2
+#define AXHIP_ROTARY_YARN 3
+AXHIP_API int axhip_rotary_inv_freq(int kind, double theta, int rotary_dim, double factor, int64_t trained_len,
+                                    double fast_turns, double slow_turns, float *inv_freq, float *scale);
+
+/* ============================================================================================
+ * New tokens of a ragged batch over a paged cache
+ *
+ * `tokens` rows in a line: those of sequence b are cu_tokens[b] .. cu_tokens[b + 1] - 1 (device int32 [B + 1], from 0,
+ * never falling; a sequence may have none), and the i-th of them sits at key position start[b] + i (device int32 [B]).
+ * Rows from cu_tokens[B] on belong to nobody: they are not read and their outputs are left as they were.  Pools and page
+ * table as for axhip_gqa_decode_paged.  All lengths are read on the device, so captured launches follow them.
+ * ========================================================================================== */
+
+/* Norm, rotation and append in one launch: per row, each q head -> RMSNorm over D (norm != 0) -> rotation (as in
+ * axhip_rotary_qk) -> q_out [tokens, Hq, D]; each k head likewise -> its row of k_pool; v heads -> their row of v_pool.
+ * q, k, v rows of `dtype` with row strides in elements (three offsets into one fused projection do); q_out and pools
+ * of `cache_dtype`; weights [D] of w_dtype or NULL; arithmetic in fp32, angles in 64 bits, one rounding at the store.
+ * pos: int64 [tokens] (pos_axes 1), int64 [3, tokens] (pos_axes 3: pair i turns by axis 1 if i % 3 == 1 and
+ * i < 3 h_sec, by axis 2 if i % 3 == 2 and i < 3 w_sec, else by axis 0), or NULL: the key position.
+ * A position outside the table and a page number outside [0, n_pages) skip the k and v rows; q is written all the same.
+ * D % 8 == 0, D <= 512, pools 16-byte aligned.  Equals rms_norm, rotation, cast and axhip_kv_append_paged in that order;
+ * the reference runs them one by one over a cache that it copies (examples/vlm/qwen3vl/model.py:353-364). */
+AXHIP_API int axhip_rotary_append_paged(const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v,
+                                        int64_t v_stride, int dtype, const void *q_weight, const void *k_weight,
+                                        int w_dtype, float eps, int norm, const int64_t *pos, int pos_axes,
+                                        const float *inv_freq, float scale, int interleaved, int rotary_dim, int h_sec,
+                                        int w_sec, const int32_t *cu_tokens, const int32_t *start,
+                                        const int32_t *page_table, void *q_out, void *k_pool, void *v_pool,
+                                        int cache_dtype, int tokens, int B, int Hq, int Hkv, int D, int max_pages,
+                                        int n_pages, axhip_stream stream);
+
+/* Causal attention of the new tokens over the cache that already holds their keys and values:
+ *   out_i = softmax(q_i . K[0 .. p]^T / sqrt(D)) V[0 .. p],  p = min(start[b] + i, max_len - 1); p < 0: zeros.
+ * From one token a sequence (decode) over drafts of a few to chunks of a prompt, mixed in one launch.
+ *   q, out [tokens, Hq, D] of `dtype` (FLOAT16 or FLOAT32), the pools' type; D 64, 128 or 256; Hq % Hkv == 0
+ *   max_q bounds every sequence's new tokens (more are not computed), max_len every p + 1; max_pages * 128 >= max_len
+ *   workspace: axhip_chunk_attention_paged_workspace_bytes(...) bytes, 16-byte aligned, contents free; launches
+ *   that may overlap in time need one each (captured graphs that replay side by side too)
+ * Page numbers outside [0, n_pages) are clamped into the pool: wrong values, never an access outside it.  Infinities and
+ * NaN in keys and values reach only rows that see them.  Same bits from run to run.
+ * Counterpart of ops::cuda::ScaledDotProductAttention with is_causal (src/ops/cuda/sequence.cu:105-163,451-472), which
+ * takes one sequence of dense tensors. */
+AXHIP_API size_t axhip_chunk_attention_paged_workspace_bytes(int dtype, int tokens, int B, int Hq, int Hkv, int D, int max_q,
+                                                             int max_len);
+AXHIP_API int axhip_chunk_attention_paged(const void *q, const void *k_pool, const void *v_pool, const int32_t *page_table,
+                                          const int32_t *cu_tokens, const int32_t *start, void *out, void *workspace,
+                                          size_t workspace_bytes, int dtype, int tokens, int B, int Hq, int Hkv, int D,
+                                          int max_q, int max_len, int max_pages, int n_pages, axhip_stream stream);
+
 /* ============================================================================================
  * fp16 Linear (cast_linear_fp16)
  * ========================================================================================== */
@@ -442,6 +517,30 @@ AXHIP_API int axhip_embedding(const void *ids, int ids_dtype, const void *table,
  * Replaces ops::cuda::ArgmaxLastDim, src/ops/cuda/sequence.cu:262-292. */
 AXHIP_API int axhip_argmax(const void *x, int64_t *out, int dtype, int64_t rows, int64_t cols,
                            axhip_stream stream);
+
+/* What a sampler does to the logits of a step before it picks a token.  For every row and token, in this order:
+ *   seen in the row's history:            x = x > 0 ? x / repetition : x * repetition
+ *   c > 0 occurrences behind the prompt:  x = x - frequency * c - presence
+ *   entries (id, value) of the bias list: x = x + (their sum, in list order; an id may stand there more than once)
+ *   mask bit not set:                     x = -inf
+ *   logits, out  [rows, vocab] of `dtype` (FLOAT16 / FLOAT32; fp32 arithmetic, one rounding), rows *_stride elements
+ *                apart; out may be logits itself
+ *   history      device int32 / int64 token ids, element (row, t) at row * history_row_stride + t * history_token_stride
+ *                (the [steps, rows] log of axhip_decode_advance: strides 1 and rows), t < history_len[row] <= max_history;
+ *                prompt_len[row]: how many of them are the prompt's.  history NULL: none; history_len NULL: max_history
+ *                each; prompt_len NULL: 0
+ *   repetition, presence, frequency  device fp32 [rows] or NULL (1, 0, 0)
+ *   bias_ids, bias  device int32 / fp32 [rows, bias_count], ids outside the vocabulary are padding
+ *   allowed      device uint32 bits, token v of a row: bit v % 32 of word v / 32; rows allowed_stride words apart; or NULL
+ * Ids outside the vocabulary are passed over.  The order of the history does not change a bit of the result.
+ * No reference counterpart (its example picks the plain argmax, examples/vlm/qwen3vl/model.py:846-858). */
+AXHIP_API int axhip_logits_process(const void *logits, int64_t logits_stride, int dtype, const void *history,
+                                   int history_dtype, int64_t history_row_stride, int64_t history_token_stride,
+                                   int max_history, const int32_t *history_len, const int32_t *prompt_len,
+                                   const float *repetition, const float *presence, const float *frequency,
+                                   const int32_t *bias_ids, const float *bias, int bias_count, const uint32_t *allowed,
+                                   int64_t allowed_stride, void *out, int64_t out_stride, int rows, int vocab,
+                                   axhip_stream stream);
 
 /* ============================================================================================
  * Glue kernels of the captured decode step (fusions of the operators above)
