@@ -35,6 +35,7 @@ constexpr int kWavesWg = 4;
 constexpr int kPageKeys = 128, kPageShift = 7;
 constexpr int kBlockKeys = 32;      // keys of one softmax step
 constexpr float kMasked = -1.0e30f;
+typedef float float8_t __attribute__((ext_vector_type(8)));
 constexpr int kMinPieceUnits = 2;   // a piece has at least 2 units of 128 keys
 
 struct ChunkArgs {
@@ -50,7 +51,7 @@ struct ChunkArgs {
 
 template <typename T, int D>
 struct Cfg {
-  static constexpr int NT = D == 256 ? 1 : 2;                          // column tiles per wavefront
+  static constexpr int NT = D == 256 || (sizeof(T) == 4 && D == 128) ? 1 : 2;  // column tiles per wavefront
   static constexpr int TR = kWavesWg * 16 * NT;                        // rows per tile
   static constexpr int FEW = 16 * NT;                                  // rows up to which wavefronts deal the keys
   static constexpr int KS = (D == 256 || (sizeof(T) == 4 && D == 128)) ? 32 : 64;  // keys per stage
@@ -142,14 +143,25 @@ __device__ __forceinline__ Piece find_piece(const ChunkArgs &a, int flat, int la
 }
 
 // ---- LDS reads of the products' operands -----------------------------------------------------------------------------
-template <int D, int SW>
-__device__ __forceinline__ half4_t v_tr(const _Float16 *stage, int key0, int d0, int c) {
-  const int key = key0 + (c >> 2);
-  const int unit = (d0 >> 3) + ((c & 3) >> 1);
-  const _Float16 *p = stage + key * D + ((unit ^ (key & SW)) << 3) + ((c & 1) << 2);
+typedef unsigned char __attribute__((address_space(3))) lds_byte;
+
+template <typename V>
+__device__ __forceinline__ V lds_at(const lds_byte *base, int offset) {
+  return *reinterpret_cast<const V __attribute__((address_space(3))) *>(base + offset);
+}
+// 4 keys x 16 d of row-major V, transposed on the way: within 16 lanes, lane i names 4 consecutive elements and receives
+// element i of each of the 4 rows.
+__device__ __forceinline__ half4_t lds_tr(const lds_byte *base, int offset) {
   typedef __fp16 fp16x4_t __attribute__((__vector_size__(4 * sizeof(__fp16))));
-  const fp16x4_t r = __builtin_amdgcn_ds_read_tr16_b64_v4f16((fp16x4_t __attribute__((address_space(3))) *)(p));
-  return __builtin_bit_cast(half4_t, r);
+  return __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((fp16x4_t __attribute__((address_space(3))) *)(base + offset)));
+}
+
+// 16 bytes a lane from memory (base, uniform, + off) straight to LDS: lane l's to dst + 16 l.
+template <typename T>
+__device__ __forceinline__ void load_lds16(const T *base, unsigned off, lds_byte *dst) {
+  const unsigned char *src = reinterpret_cast<const unsigned char *>(base) + off;
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                   (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
 }
 
 // Whether a 16-byte unit holds an infinity or a NaN, and the unit without them.
@@ -194,7 +206,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
   constexpr int DT = D / 16;
   constexpr int QF = sizeof(T) == 2 ? D / 32 : D / 4;  // operand registers of a column tile (8 halves or 1 float each)
   constexpr bool kHalf = sizeof(T) == 2;
-  S *ks = reinterpret_cast<S *>(chunk_smem), *vs = ks + 2 * KS * D;
+  constexpr int kRow = D * static_cast<int>(sizeof(T)), kTensor = 2 * KS * kRow;  // bytes: a row, both stages of K (V behind)
+  lds_byte *smem = (lds_byte *)chunk_smem;
   int *s_flag = reinterpret_cast<int *>(chunk_smem + C::kLdsBytes - 16);
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -227,53 +240,55 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
   // infinities and NaN of V are stored as zeros too (0 * inf is NaN) and added at the end to the rows that see them
   const int mixed_from = tile_first < 0 ? 0 : (tile_first + 1) / KS * KS;
 
-  // element offset of this thread's units within a page, and in a stage's LDS
-  unsigned voff[VEC];
-  int lds_o[VEC];
-#pragma unroll
-  for (int p = 0; p < VEC; ++p) {
-    const int vi = p * kThreads + tid, row = vi / UPR, unit = vi % UPR;
-    voff[p] = row * D + unit * C::E;
-    lds_o[p] = row * D + ((unit ^ (row & SW)) * C::E);
-  }
-  const int32_t *table = a.page_table + static_cast<int64_t>(pc.b) * a.max_pages;
+  // K and V go from memory to LDS directly (16 bytes a lane; a wavefront fills 1 KiB in lane order, so the swizzle is made on
+  // the side of memory: the lane of place u of a row fetches unit u ^ (row & SW)).  Load p of a thread covers row
+  // p kStep + tid / UPR of the stage; its offset within the page differs by constants from load 0's.
+  constexpr int kStep = kThreads / UPR;
+  const unsigned voff = tid / UPR * kRow + ((tid % UPR) ^ ((tid / UPR) & SW)) * 16;
+  // Where this lane reads its operands, as byte offsets into a stage of K / V; the steps of the products flip or add constant
+  // bits of them.  Made opaque in every block, or the compiler keeps every one of the flipped offsets in registers.
+  const int kaddr = c * kRow + (kHalf ? (g ^ (c & SW)) * 16 : (c & SW) * 16 + g * 4);
+  const int vkey = kHalf ? 4 * g + (c >> 2) : 4 * g;
+  const int vaddr = vkey * kRow + (kHalf ? ((((c & 3) >> 1) ^ (vkey & SW)) * 16 + (c & 1) * 8) : (((c >> 2) ^ (vkey & SW)) * 16 + (c & 3) * 4));
+  // page numbers by scalar loads: a vector load would have to be waited for behind the stage on its way
+  typedef const int32_t __attribute__((address_space(4))) *scalar_ptr;
+  const scalar_ptr table = (scalar_ptr)(a.page_table + static_cast<int64_t>(pc.b) * a.max_pages);
   const int64_t page_elems = static_cast<int64_t>(a.Hkv) * kPageKeys * D;
   const T *kbase = static_cast<const T *>(a.k) + static_cast<int64_t>(hk) * kPageKeys * D;
   const T *vbase = static_cast<const T *>(a.v) + static_cast<int64_t>(hk) * kPageKeys * D;
-  auto page_at = [&](int key) { return min(max(table[key >> kPageShift], 0), a.n_pages - 1); };  // never outside the pool
-  u32x4_t kst[VEC], vst[VEC];
-  auto load_stage = [&](int page, int key0) __attribute__((always_inline)) {
-    const int64_t base = page * page_elems + static_cast<int64_t>(key0 & (kPageKeys - 1)) * D;
-    const T *kb = kbase + base, *vb = vbase + base;
+  auto in_pool = [&](int page) { return min(max(page, 0), a.n_pages - 1); };
+  auto load_stage = [&](int page, int key0, int buf) __attribute__((always_inline)) {
+    const int64_t base = in_pool(page) * page_elems + static_cast<int64_t>(key0 & (kPageKeys - 1)) * D;
+    const unsigned place = buf * (KS * kRow) + wave * 1024;
 #pragma unroll
     for (int p = 0; p < VEC; ++p) {
-      kst[p] = *reinterpret_cast<const u32x4_t *>(kb + voff[p]);
-      vst[p] = *reinterpret_cast<const u32x4_t *>(vb + voff[p]);
+      const unsigned off = (voff ^ ((p * kStep & SW) * 16)) + p * kStep * kRow;
+      load_lds16(kbase + base, off, smem + place + p * kThreads * 16);
+      load_lds16(vbase + base, off, smem + kTensor + place + p * kThreads * 16);
     }
   };
-  auto store_stage = [&](int buf, int key0) __attribute__((always_inline)) {
-    S *kd = ks + buf * KS * D, *vd = vs + buf * KS * D;
+  // The units that this thread has fetched are in LDS.  (In its own order: the barrier behind this call makes them everybody's.)
+  auto stage_arrived = [&](int key0, int buf) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (key0 + KS > mixed_from) {  // uniform; also every stage that reaches past k_end, for mixed_from <= k_all
       bool bad = false;
-#pragma unroll
+#pragma unroll 1
       for (int p = 0; p < VEC; ++p) {
-        const int row = (p * kThreads + tid) / UPR;
-        if (key0 + row >= k_end) vst[p] = u32x4_t{0, 0, 0, 0};
-        if (unit_bad<T>(vst[p])) {
+        typedef u32x4_t __attribute__((address_space(3))) lds_unit;
+        lds_unit *at = reinterpret_cast<lds_unit *>(smem + kTensor + buf * (KS * kRow) + (p * kThreads + tid) * 16);
+        u32x4_t u = *at;
+        if (key0 + p * kStep + tid / UPR >= k_end) {
+          *at = u32x4_t{0, 0, 0, 0};
+        } else if (unit_bad<T>(u)) {
           bad = true;
-          vst[p] = unit_finite<T>(vst[p]);
+          *at = unit_finite<T>(u);
         }
       }
       if (bad) *s_flag = 1;
     }
-#pragma unroll
-    for (int p = 0; p < VEC; ++p) {
-      *reinterpret_cast<u32x4_t *>(kd + lds_o[p]) = kst[p];
-      *reinterpret_cast<u32x4_t *>(vd + lds_o[p]) = vst[p];
-    }
   };
 
-  if (n_stages > 0) load_stage(page_at(k0), k0);
+  if (n_stages > 0) load_stage(table[k0 >> kPageShift], k0, 0);
 
   // Q as the right operand of the first product, for the whole kernel
   typename std::conditional<kHalf, half8_t, float>::type qf[NT][QF];
@@ -299,9 +314,12 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
     for (int dt = 0; dt < DT; ++dt) o[t][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
 
-  // one block of 32 keys kb .. kb + 31 at rows k_l / v_l of a stage.  MASK: some key of it is behind some row's position
-  auto block = [&](const S *k_l, const S *v_l, int kb, auto mask_c) __attribute__((always_inline)) {
+  // one block of 32 keys kb .. kb + 31, block `sub` of stage buffer `buf`.  MASK: some key of it is behind some row's position
+  auto block = [&](int buf, int sub, int kb, auto mask_c) __attribute__((always_inline)) {
     constexpr bool MASK = decltype(mask_c)::value;
+    const lds_byte *k_l = smem + sub * (kBlockKeys * kRow), *v_l = k_l + kTensor;
+    int ka = kaddr + buf * (KS * kRow), va = vaddr + buf * (KS * kRow);
+    asm volatile("" : "+v"(ka), "+v"(va));
     float4_t sc[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -309,18 +327,17 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
     for (int tk = 0; tk < 2; ++tk)
 #pragma unroll
       for (int kk = 0; kk < QF; ++kk) {
-        const int row = tk * 16 + c;  // row & 15 == c
         if constexpr (kHalf) {
-          const half8_t kf = lds_h8(k_l + row * D + (((kk * 4 + g) ^ (c & SW)) << 3));
+          const half8_t kf = lds_at<half8_t>(k_l, (ka ^ (kk * 64)) + tk * 16 * kRow);
 #pragma unroll
           for (int t = 0; t < NT; ++t) sc[t][tk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[t][kk], sc[t][tk], 0, 0, 0);
         } else {
-          const float kf = k_l[row * D + ((kk ^ (c & SW)) << 2) + g];
+          const float kf = lds_at<float>(k_l, (ka ^ (kk * 16)) + tk * 16 * kRow);
 #pragma unroll
           for (int t = 0; t < NT; ++t) sc[t][tk] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf, qf[t][kk], sc[t][tk], 0, 0, 0);
         }
       }
-    float pr[NT][8];
+    typename std::conditional<kHalf, half8_t, float8_t>::type pf[NT];
     bool moved[NT];
     float mnew[NT];
 #pragma unroll
@@ -347,7 +364,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
       for (int j = 0; j < 8; ++j) {
         float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], a.scale_log2e, -mnew[t]));
         if (MASK && x[j] <= kMasked) p = 0.f;  // a row that has seen no key keeps m = kMasked: exp2(0) would count
-        pr[t][j] = p;
+        if constexpr (kHalf) pf[t][j] = static_cast<_Float16>(p);
+        else pf[t][j] = p;
       }
     }
 #pragma unroll
@@ -361,19 +379,13 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
       }
     }
     if constexpr (kHalf) {
-      half8_t pf[NT];
       const half8_t ones = {1, 1, 1, 1, 1, 1, 1, 1};
+      // the row sums as a product with ones: every register of the result holds the row's sum
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) pf[t][j] = static_cast<_Float16>(pr[t][j]);
-        // the row sums as a product with ones: every register of the result holds the row's sum
-        lsum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[t], lsum[t], 0, 0, 0);
-      }
+      for (int t = 0; t < NT; ++t) lsum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[t], lsum[t], 0, 0, 0);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const half4_t lo = v_tr<D, SW>(v_l, 4 * g, dt * 16, c);
-        const half4_t hi = v_tr<D, SW>(v_l, 16 + 4 * g, dt * 16, c);
+        const half4_t lo = lds_tr(v_l, va ^ (dt * 32)), hi = lds_tr(v_l, (va ^ (dt * 32)) + 16 * kRow);
         const half8_t vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
         for (int t = 0; t < NT; ++t) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[t], o[t][dt], 0, 0, 0);
@@ -384,14 +396,13 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
       for (int tk = 0; tk < 2; ++tk)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int row = tk * 16 + 4 * g + e;
 #pragma unroll
-          for (int t = 0; t < NT; ++t) lsum[t][0] += pr[t][tk * 4 + e];
+          for (int t = 0; t < NT; ++t) lsum[t][0] += pf[t][tk * 4 + e];
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
-            const float vf = v_l[row * D + (((dt * 4 + (c >> 2)) ^ (row & SW)) << 2) + (c & 3)];
+            const float vf = lds_at<float>(v_l, (va ^ (dt * 64) ^ (e * 16)) + (tk * 16 + e) * kRow);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, pr[t][tk * 4 + e], o[t][dt], 0, 0, 0);
+            for (int t = 0; t < NT; ++t) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, pf[t][tk * 4 + e], o[t][dt], 0, 0, 0);
           }
         }
     }
@@ -399,29 +410,28 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
 
   if (n_stages > 0) {
     __syncthreads();  // the flag is cleared
-    store_stage(0, k0);
-    __syncthreads();
-    int page = page_at(min(k0 + KS, k_end - 1));
+    stage_arrived(k0, 0);
+    lds_barrier();
+    int page = table[min(k0 + KS, k_end - 1) >> kPageShift];  // of the next stage
     for (int s = 0; s < n_stages; ++s) {
       const int buf = s & 1, key0 = k0 + s * KS;
-      const int nxt = k0 + min(s + 1, n_stages - 1) * KS;  // the last stage fetches itself again: no branch
-      load_stage(page, nxt);
-      page = page_at(k0 + min(s + 2, n_stages - 1) * KS);
+      const bool more = s + 1 < n_stages;
+      if (more) load_stage(page, key0 + KS, buf ^ 1);  // everybody has left that buffer
+      page = table[min(key0 + 2 * KS, k_end - 1) >> kPageShift];
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int sub = 0; sub < KS / kBlockKeys; ++sub) {
         const int kb = key0 + sub * kBlockKeys;
         const bool mine = few ? sub == wave : !idle;
         if (mine && kb <= wave_last && kb < k_end) {  // wave-uniform
-          const S *k_l = ks + (buf * KS + sub * kBlockKeys) * D, *v_l = vs + (buf * KS + sub * kBlockKeys) * D;
-          if (kb + kBlockKeys - 1 > wave_first) block(k_l, v_l, kb, std::true_type{});
-          else block(k_l, v_l, kb, std::false_type{});
+          if (kb + kBlockKeys - 1 > wave_first) block(buf, sub, kb, std::true_type{});
+          else block(buf, sub, kb, std::false_type{});
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-      if (s + 1 < n_stages) {
-        store_stage(buf ^ 1, nxt);
-        __syncthreads();
+      if (more) {
+        stage_arrived(key0 + KS, buf ^ 1);
+        lds_barrier();
       }
     }
   }
@@ -432,17 +442,6 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
   __syncthreads();
   const bool repair = *s_flag != 0;  // uniform
 
-  // infinities and NaN of V that were stored as zeros: added to element d of every row that sees their key (a positive
-  // weight does not change them)
-  auto nonfinite_sum = [&](int d, int last) {
-    float sum = 0.f;
-    for (int key = max(k0, mixed_from); key < k_end && key <= last; ++key) {
-      const int64_t off = page_at(key) * page_elems + static_cast<int64_t>(key & (kPageKeys - 1)) * D + d;
-      const float x = ldf(vbase + off);
-      if (!(fabsf(x) < __builtin_inff())) sum += x;
-    }
-    return sum;
-  };
   const bool cut = pc.pieces > 1;
   const int64_t slot = static_cast<int64_t>(pc.slot) * a.Hkv + hk;
   if (cut && (slot >= a.slots || n_rows > a.slot_rows)) return;  // (cannot happen: the cut is bounded by both)
@@ -451,17 +450,30 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
     return static_cast<T *>(a.out) + (static_cast<int64_t>(pc.c0 + i) * a.Hq + hk * a.group + (rr - i * a.group)) * D;
   };
 
+  // Infinities and NaN of V that were stored as zeros are added at the end, to element d of every row that sees their key
+  // (a positive weight does not change them): rare, so through memory and without a thought for speed.
+  auto finish = [&]() {
+    if (!repair) return;
+    __threadfence_block();
+    __syncthreads();
+    for (int x = tid; x < n_rows * D; x += kThreads) {
+      const int r = x / D, d = x % D, last = position(r);
+      float sum = 0.f;
+      for (int key = max(k0, mixed_from); key < k_end && key <= last; ++key) {
+        const float v = ldf(vbase + in_pool(table[key >> kPageShift]) * page_elems + static_cast<int64_t>(key & (kPageKeys - 1)) * D + d);
+        if (!(fabsf(v) < __builtin_inff())) sum += v;
+      }
+      if (sum == 0.f) continue;
+      if (cut) a.part_o[(slot * a.slot_rows + r) * D + d] += sum;
+      else stf(out_row(r) + d, ldf(out_row(r) + d) + sum);
+    }
+  };
+
   if (!few) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int r = wrow + t * 16 + c;
       if (r >= n_rows) continue;
-      if (repair) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[t][dt][e] += nonfinite_sum(dt * 16 + 4 * g + e, pos[t]);
-      }
       const float l = lsum[t][0];
       if (cut) {
         float *po = a.part_o + (slot * a.slot_rows + r) * D;
@@ -484,6 +496,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
         }
       }
     }
+    finish();
     return;
   }
 
@@ -515,7 +528,6 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
       l = __builtin_fmaf(f, sml[2 * (w * C::FEW + r) + 1], l);
       acc = add_weighted(acc, f, so[(w * C::FEW + r) * C::STATE + d]);
     }
-    if (repair) acc += nonfinite_sum(d, position(r));
     if (cut) {
       a.part_o[(slot * a.slot_rows + r) * D + d] = acc;
       if (d == 0) {
@@ -527,6 +539,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
       stf(out_row(r) + d, acc * inv);
     }
   }
+  finish();
 }
 
 // Adds the pieces of a cut tile: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), in the order of the keys.
@@ -594,7 +607,7 @@ Sizes sizes_for(int tile_rows, int tokens, int B, int Hkv, int group, int max_q,
   }
   return z;
 }
-int tile_rows_of(int D) { return D == 256 ? 64 : 128; }
+int tile_rows_of(int dtype, int D) { return D == 256 || (dtype == AXHIP_FLOAT32 && D == 128) ? 64 : 128; }
 
 template <typename T, int D>
 int launch(const ChunkArgs &a, const Sizes &z, hipStream_t st) {
@@ -632,7 +645,7 @@ AXHIP_API size_t axhip_chunk_attention_paged_workspace_bytes(int dtype, int toke
                                                              int max_len) {
   if (check_sizes(dtype, tokens, B, Hq, Hkv, D, max_q, max_len) != AXHIP_OK) return 0;
   if (max_q > tokens) max_q = tokens;
-  const Sizes z = sizes_for(tile_rows_of(D), tokens, B, Hkv, Hq / Hkv, max_q, max_len);
+  const Sizes z = sizes_for(tile_rows_of(dtype, D), tokens, B, Hkv, Hq / Hkv, max_q, max_len);
   return static_cast<size_t>(z.slots) * z.slot_rows * (D + 2) * sizeof(float);
 }
 
@@ -650,7 +663,7 @@ AXHIP_API int axhip_chunk_attention_paged(const void *q, const void *k_pool, con
     return AXHIP_INVALID_PTR;
   if (max_q > tokens) max_q = tokens;
   const int group = Hq / Hkv;
-  const Sizes z = sizes_for(tile_rows_of(D), tokens, B, Hkv, group, max_q, max_len);
+  const Sizes z = sizes_for(tile_rows_of(dtype, D), tokens, B, Hkv, group, max_q, max_len);
   const size_t need = static_cast<size_t>(z.slots) * z.slot_rows * (D + 2) * sizeof(float);
   if (need && (!workspace || !aligned_to(workspace, 16))) return AXHIP_INVALID_PTR;
   if (workspace_bytes < need) return AXHIP_OUT_OF_MEMORY;
