@@ -314,84 +314,111 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
     for (int dt = 0; dt < DT; ++dt) o[t][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
   }
 
-  // one block of 32 keys kb .. kb + 31, block `sub` of stage buffer `buf`.  MASK: some key of it is behind some row's position
-  auto block = [&](int buf, int sub, int kb, auto mask_c) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(mask_c)::value;
-    const lds_byte *k_l = smem + sub * (kBlockKeys * kRow), *v_l = k_l + kTensor;
-    int ka = kaddr + buf * (KS * kRow), va = vaddr + buf * (KS * kRow);
-    asm volatile("" : "+v"(ka), "+v"(va));
-    float4_t sc[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = float4_t{0.f, 0.f, 0.f, 0.f};
+  // ---- a block of 32 keys for this wavefront, in four parts ------------------------------------------------------------
+  using KFrag = typename std::conditional<kHalf, half8_t, float>::type;
+  using Probs = typename std::conditional<kHalf, half8_t, float8_t>::type;
+  auto read_k = [&](int buf, int sub, KFrag (&kf)[2][QF]) __attribute__((always_inline)) {
+    const lds_byte *k_l = smem + sub * (kBlockKeys * kRow);
+    int ka = kaddr + buf * (KS * kRow);
+    asm volatile("" : "+v"(ka));
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk)
 #pragma unroll
-      for (int kk = 0; kk < QF; ++kk) {
-        if constexpr (kHalf) {
-          const half8_t kf = lds_at<half8_t>(k_l, (ka ^ (kk * 64)) + tk * 16 * kRow);
+      for (int kk = 0; kk < QF; ++kk) kf[tk][kk] = lds_at<KFrag>(k_l, (ka ^ (kk * (kHalf ? 64 : 16))) + tk * 16 * kRow);
+  };
+  auto scores = [&](const KFrag (&kf)[2][QF], float4_t (&sc)[NT][2]) __attribute__((always_inline)) {
 #pragma unroll
-          for (int t = 0; t < NT; ++t) sc[t][tk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[t][kk], sc[t][tk], 0, 0, 0);
-        } else {
-          const float kf = lds_at<float>(k_l, (ka ^ (kk * 16)) + tk * 16 * kRow);
+    for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int t = 0; t < NT; ++t) sc[t][tk] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf, qf[t][kk], sc[t][tk], 0, 0, 0);
-        }
-      }
-    typename std::conditional<kHalf, half8_t, float8_t>::type pf[NT];
-    bool moved[NT];
-    float mnew[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float x[8];
+    for (int kk = 0; kk < QF; ++kk)
 #pragma unroll
       for (int tk = 0; tk < 2; ++tk)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = sc[t][tk][e];
-          if (MASK && kb + tk * 16 + 4 * g + e > pos[t]) v = kMasked;
-          x[tk * 4 + e] = v;
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (kHalf) sc[t][tk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tk][kk], qf[t][kk], sc[t][tk], 0, 0, 0);
+          else sc[t][tk] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[tk][kk], qf[t][kk], sc[t][tk], 0, 0, 0);
         }
-      float mx = x[0];
+  };
+  // Probabilities against the running maximum as it stands: it is moved, and everything rescaled, only when one of them
+  // passes 2^8 (the first block of a row always does).  Until then p <= 256, which fp16 holds to the same 11 bits, and a
+  // block needs no maximum over its row at all.  (The maximum never runs ahead, so no p is smaller than against the true one.)
+  // MASK: some key of the block at kb is behind some row's position.
+  auto softmax = [&](const float4_t (&sc)[NT][2], Probs (&pf)[NT], int kb, auto mask_c) __attribute__((always_inline)) {
+    constexpr bool MASK = decltype(mask_c)::value;
+    float p[NT][8];
+    auto x_at = [&](int t, int j) __attribute__((always_inline)) {
+      float v = sc[t][j >> 2][j & 3];
+      if (MASK && kb + (j >> 2) * 16 + 4 * g + (j & 3) > pos[t]) v = kMasked;
+      return v;
+    };
+    auto exps = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 1; j < 8; ++j) mx = fmaxf(mx, x[j]);
-      mx = max_xor32(max_xor16(mx));
-      // the running maximum moves only past a factor 2^8: until then p <= 256, which fp16 holds to the same 11 bits,
-      // and nothing is rescaled
-      const float mxs = mx * a.scale_log2e;
-      moved[t] = __any(mxs > m[t] + 8.0f);
-      mnew[t] = moved[t] ? fmaxf(m[t], mxs) : m[t];
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], a.scale_log2e, -mnew[t]));
-        if (MASK && x[j] <= kMasked) p = 0.f;  // a row that has seen no key keeps m = kMasked: exp2(0) would count
-        if constexpr (kHalf) pf[t][j] = static_cast<_Float16>(p);
-        else pf[t][j] = p;
-      }
-    }
+        for (int j = 0; j < 8; ++j) {
+          const float x = x_at(t, j);
+          p[t][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.scale_log2e, -m[t]));
+          if (MASK && x <= kMasked) p[t][j] = 0.f;
+        }
+    };
+    exps();
+    float top = 0.f;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (moved[t]) {
-        const float corr = __builtin_amdgcn_exp2f(m[t] - mnew[t]);
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = fmaxf(top, p[t][j]);
+    if (__builtin_expect(__any(top > 256.f), 0)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float mx = x_at(t, 0);
+#pragma unroll
+        for (int j = 1; j < 8; ++j) mx = fmaxf(mx, x_at(t, j));
+        const float mnew = fmaxf(m[t], max_xor32(max_xor16(mx)) * a.scale_log2e);
+        const float corr = __builtin_amdgcn_exp2f(m[t] - mnew);
+        m[t] = mnew;
         lsum[t] *= corr;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[t][dt] *= corr;
-        m[t] = mnew[t];
       }
+      exps();
     }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (kHalf) pf[t][j] = static_cast<_Float16>(p[t][j]);
+        else pf[t][j] = p[t][j];
+      }
+  };
+  // fp16: V^T fragments of the block, d tile by d tile
+  auto read_v = [&](int buf, int sub, half8_t (&vf)[DT]) __attribute__((always_inline)) {
+    const lds_byte *v_l = smem + sub * (kBlockKeys * kRow) + kTensor;
+    int va = vaddr + buf * (KS * kRow);
+    asm volatile("" : "+v"(va));
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const half4_t lo = lds_tr(v_l, va ^ (dt * 32)), hi = lds_tr(v_l, (va ^ (dt * 32)) + 16 * kRow);
+      vf[dt] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  };
+  auto add_values = [&](const half8_t (&vf)[DT], const Probs (&pf)[NT]) __attribute__((always_inline)) {
     if constexpr (kHalf) {
       const half8_t ones = {1, 1, 1, 1, 1, 1, 1, 1};
       // the row sums as a product with ones: every register of the result holds the row's sum
 #pragma unroll
       for (int t = 0; t < NT; ++t) lsum[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[t], lsum[t], 0, 0, 0);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const half4_t lo = lds_tr(v_l, va ^ (dt * 32)), hi = lds_tr(v_l, (va ^ (dt * 32)) + 16 * kRow);
-        const half8_t vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[t], o[t][dt], 0, 0, 0);
-      }
-    } else {
-      // product step (tk, e) takes keys tk * 16 + 4 g + e, g = 0 .. 3: the score register e of a lane is its right operand
+        for (int t = 0; t < NT; ++t) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[dt], pf[t], o[t][dt], 0, 0, 0);
+    }
+  };
+  // fp32: product step (tk, e) takes keys tk * 16 + 4 g + e, g = 0 .. 3, so that a lane's score register e is its right operand
+  auto add_values_f32 = [&](int buf, int sub, const Probs (&pf)[NT]) __attribute__((always_inline)) {
+    if constexpr (!kHalf) {
+      const lds_byte *v_l = smem + sub * (kBlockKeys * kRow) + kTensor;
+      int va = vaddr + buf * (KS * kRow);
+      asm volatile("" : "+v"(va));
 #pragma unroll
       for (int tk = 0; tk < 2; ++tk)
 #pragma unroll
@@ -407,18 +434,75 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
         }
     }
   };
+  auto block = [&](int buf, int sub, int kb, auto mask_c) __attribute__((always_inline)) {
+    KFrag kf[2][QF];
+    float4_t sc[NT][2];
+    Probs pf[NT];
+    read_k(buf, sub, kf);
+    scores(kf, sc);
+    softmax(sc, pf, kb, mask_c);
+    if constexpr (kHalf) {
+      half8_t vf[DT];
+      read_v(buf, sub, vf);
+      add_values(vf, pf);
+    } else {
+      add_values_f32(buf, sub, pf);
+    }
+  };
 
+  // ---- the stages -------------------------------------------------------------------------------------------------------
+  // At the top of stage s its keys are in buffer s & 1 for everybody and stage s + 1 is on its way into the other buffer.
   if (n_stages > 0) {
     __syncthreads();  // the flag is cleared
     stage_arrived(k0, 0);
     lds_barrier();
-    int page = table[min(k0 + KS, k_end - 1) >> kPageShift];  // of the next stage
-    for (int s = 0; s < n_stages; ++s) {
+    if (n_stages > 1) load_stage(table[(k0 + KS) >> kPageShift], k0 + KS, 1);
+    auto page_after = [&](int s) { return table[min(k0 + (s + 2) * KS, k_end - 1) >> kPageShift]; };
+    int s = 0, page = page_after(0);
+    // Stages that every row of the tile sees whole run as a software pipeline: while one block's scores and values are
+    // multiplied, the next operands come from LDS, so a wavefront never waits for an LDS read that it has just made.  The
+    // barrier that ends a stage stands in the middle of its last block, behind that block's last LDS read.
+    if constexpr (kHalf && KS == 2 * kBlockKeys) {
+      const int n_fast = few || tile_first < k0 ? 0 : min((tile_first + 1 - k0) / KS, n_stages);
+      if (n_fast > 0) {
+        KFrag kf[2][QF];
+        if (!idle) read_k(0, 0, kf);
+        for (; s < n_fast; ++s) {
+          const int buf = s & 1, key0 = k0 + s * KS;
+          const bool more = s + 1 < n_stages;
+          half8_t vf[DT];
+          float4_t sc[NT][2];
+          Probs pf[NT];
+          if (!idle) {
+            scores(kf, sc);
+            read_v(buf, 0, vf);
+            read_k(buf, 1, kf);
+            __builtin_amdgcn_sched_barrier(0);
+            softmax(sc, pf, key0, std::false_type{});
+            add_values(vf, pf);
+            __builtin_amdgcn_sched_barrier(0);
+            scores(kf, sc);
+            read_v(buf, 1, vf);
+          }
+          if (more) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            stage_arrived(key0 + KS, buf ^ 1);
+            lds_barrier();
+            if (s + 2 < n_stages) load_stage(page, key0 + 2 * KS, buf);
+            page = page_after(s + 1);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          if (!idle) {
+            if (s + 1 < n_fast) read_k(buf ^ 1, 0, kf);
+            softmax(sc, pf, key0, std::false_type{});
+            add_values(vf, pf);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    for (; s < n_stages; ++s) {
       const int buf = s & 1, key0 = k0 + s * KS;
-      const bool more = s + 1 < n_stages;
-      if (more) load_stage(page, key0 + KS, buf ^ 1);  // everybody has left that buffer
-      page = table[min(key0 + 2 * KS, k_end - 1) >> kPageShift];
-      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int sub = 0; sub < KS / kBlockKeys; ++sub) {
         const int kb = key0 + sub * kBlockKeys;
@@ -428,10 +512,11 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
           else block(buf, sub, kb, std::false_type{});
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
-      if (more) {
+      if (s + 1 < n_stages) {
         stage_arrived(key0 + KS, buf ^ 1);
         lds_barrier();
+        if (s + 2 < n_stages) load_stage(page, key0 + 2 * KS, buf);
+        page = page_after(s + 1);
       }
     }
   }
