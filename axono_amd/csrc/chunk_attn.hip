@@ -61,7 +61,8 @@ struct Cfg {
   static constexpr int VEC = KS * UPR / kThreads;                      // units per thread, tensor and stage
   static constexpr int STATE = D + 4;                                  // row stride of the states added up in LDS
   static constexpr int kStageBytes = 4 * KS * D * static_cast<int>(sizeof(T));
-  static constexpr int kDealt = KS / kBlockKeys < kWavesWg ? KS / kBlockKeys : kWavesWg;  // wavefronts with keys of their own
+  // wavefronts with keys of their own in a tile of few rows
+  static constexpr int kDealt = sizeof(T) == 2 && D <= 128 ? kWavesWg : (KS / kBlockKeys < kWavesWg ? KS / kBlockKeys : kWavesWg);
   static constexpr int kStateBytes = kDealt * FEW * (STATE + 2) * 4;
   static constexpr int kLdsBytes = (kStageBytes > kStateBytes ? kStageBytes : kStateBytes) + 16;
 };
@@ -156,12 +157,12 @@ __device__ __forceinline__ half4_t lds_tr(const lds_byte *base, int offset) {
   return __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((fp16x4_t __attribute__((address_space(3))) *)(base + offset)));
 }
 
-// 16 bytes a lane from memory (base, uniform, + off) straight to LDS: lane l's to dst + 16 l.
-template <typename T>
+// 16 bytes a lane from memory (base, uniform, + off) straight to LDS: lane l's to dst + 16 l.  AUX 2: a non-temporal load.
+template <typename T, int AUX = 0>
 __device__ __forceinline__ void load_lds16(const T *base, unsigned off, lds_byte *dst) {
   const unsigned char *src = reinterpret_cast<const unsigned char *>(base) + off;
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
-                                   (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+                                   (__attribute__((address_space(3))) void *)dst, 16, 0, AUX);
 }
 
 // Whether a 16-byte unit holds an infinity or a NaN, and the unit without them.
@@ -267,28 +268,33 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
       load_lds16(vbase + base, off, smem + kTensor + place + p * kThreads * 16);
     }
   };
+  // V of key `key` in LDS: zeros behind the piece, no infinities and NaN; whether there were any.
+  auto clean_unit = [&](lds_byte *place, int key) __attribute__((always_inline)) {
+    typedef u32x4_t __attribute__((address_space(3))) lds_unit;
+    lds_unit *at = reinterpret_cast<lds_unit *>(place);
+    const u32x4_t u = *at;
+    if (key >= k_end) {
+      *at = u32x4_t{0, 0, 0, 0};
+    } else if (unit_bad<T>(u)) {
+      *at = unit_finite<T>(u);
+      return true;
+    }
+    return false;
+  };
   // The units that this thread has fetched are in LDS.  (In its own order: the barrier behind this call makes them everybody's.)
   auto stage_arrived = [&](int key0, int buf) __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (key0 + KS > mixed_from) {  // uniform; also every stage that reaches past k_end, for mixed_from <= k_all
       bool bad = false;
 #pragma unroll 1
-      for (int p = 0; p < VEC; ++p) {
-        typedef u32x4_t __attribute__((address_space(3))) lds_unit;
-        lds_unit *at = reinterpret_cast<lds_unit *>(smem + kTensor + buf * (KS * kRow) + (p * kThreads + tid) * 16);
-        u32x4_t u = *at;
-        if (key0 + p * kStep + tid / UPR >= k_end) {
-          *at = u32x4_t{0, 0, 0, 0};
-        } else if (unit_bad<T>(u)) {
-          bad = true;
-          *at = unit_finite<T>(u);
-        }
-      }
+      for (int p = 0; p < VEC; ++p)
+        bad |= clean_unit(smem + kTensor + buf * (KS * kRow) + (p * kThreads + tid) * 16, key0 + p * kStep + tid / UPR);
       if (bad) *s_flag = 1;
     }
   };
 
-  if (n_stages > 0) load_stage(table[k0 >> kPageShift], k0, 0);
+  const bool own_blocks = few && kHalf && D <= 128;
+  if (n_stages > 0 && !own_blocks) load_stage(table[k0 >> kPageShift], k0, 0);
 
   // Q as the right operand of the first product, for the whole kernel
   typename std::conditional<kHalf, half8_t, float>::type qf[NT][QF];
@@ -450,9 +456,93 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
     }
   };
 
+  // ---- a tile with few rows, fp16 ------------------------------------------------------------------------------------------
+  // Bound by the stream of keys, so every wavefront takes blocks of its own (block i of the piece goes to wavefront i % 4) and
+  // waits for nobody: K goes to registers in operand order (16 rows x 64 bytes a load), V through a strip of LDS of the
+  // wavefront's own, both a block ahead, read once and therefore past the caches.
+  constexpr bool kOwnBlocks = kHalf && D <= 128;
+  auto few_rows = [&]() __attribute__((always_inline)) {
+    constexpr int kVBytes = kBlockKeys * kRow, kLoads = kVBytes / 1024;  // V of a block; loads of a lane for it, as many for K
+    constexpr int kRowsALoad = 1024 / kRow;
+    static_assert(!kOwnBlocks || 2 * kWavesWg * kVBytes <= C::kStageBytes, "two blocks of V per wavefront fit the stages' LDS");
+    auto fetch = [&](int page, int kb, int buf, KFrag (&kf)[2][QF]) __attribute__((always_inline)) {
+      const int64_t base = in_pool(page) * page_elems + static_cast<int64_t>(kb & (kPageKeys - 1)) * D;
+      int l = lane;
+      asm volatile("" : "+v"(l));  // offsets are made here, not kept
+      const unsigned v_row = static_cast<unsigned>(l) / UPR, v_off = v_row * kRow + ((l % UPR) ^ (v_row & SW)) * 16;
+#pragma unroll
+      for (int p = 0; p < kLoads; ++p)
+        load_lds16<T, 2>(vbase + base, (v_off ^ ((p * kRowsALoad & SW) * 16)) + p * 1024, smem + (wave * 2 + buf) * kVBytes + p * 1024);
+      const T *kb_ = kbase + base + (l & 15) * D + (l >> 4) * 8;
+#pragma unroll
+      for (int tk = 0; tk < 2; ++tk)
+#pragma unroll
+        for (int kk = 0; kk < QF; ++kk)
+          if constexpr (kHalf)
+            kf[tk][kk] = __builtin_bit_cast(half8_t, __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(kb_ + tk * 16 * D + kk * 32)));
+    };
+    auto use = [&](int kb, int buf, const KFrag (&kf)[2][QF]) __attribute__((always_inline)) {
+      float4_t sc[NT][2];
+      Probs pf[NT];
+      scores(kf, sc);
+      __builtin_amdgcn_sched_barrier(0);
+      if (kb + kBlockKeys > mixed_from) {
+#pragma unroll 1
+        for (int p = 0; p < kLoads; ++p)
+          if (clean_unit(smem + (wave * 2 + buf) * kVBytes + p * 1024 + lane * 16, kb + static_cast<int>(lane / UPR) + p * kRowsALoad)) *s_flag = 1;
+      }
+      softmax(sc, pf, kb, std::true_type{});
+      __builtin_amdgcn_sched_barrier(0);
+      half8_t vf[DT];
+      int va = vaddr + (wave * 2 + buf) * kVBytes;
+      asm volatile("" : "+v"(va));
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const half4_t lo = lds_tr(smem, va ^ (dt * 32)), hi = lds_tr(smem, (va ^ (dt * 32)) + 16 * kRow);
+        vf[dt] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+      add_values(vf, pf);
+    };
+    constexpr int kHop = kWavesWg * kBlockKeys;  // 128 keys: the wavefront's next block lies in the next page
+    KFrag k_a[2][QF], k_b[2][QF];
+    int kb = k0 + wave * kBlockKeys;
+    if (kb >= k_end) return;
+    auto page_of = [&](int key) { return table[min(key, k_end - 1) >> kPageShift]; };
+    fetch(page_of(kb), kb, 0, k_a);
+    int page = page_of(kb + kHop);
+    // the loads of the block in use have arrived when no more than the next block's are under way (loads return in order)
+    while (true) {
+      if (kb + kHop < k_end) {
+        fetch(page, kb + kHop, 1, k_b);
+        page = page_of(kb + 2 * kHop);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      use(kb, 0, k_a);
+      kb += kHop;
+      if (kb >= k_end) break;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V of the block just used is in registers: its strip is free
+      if (kb + kHop < k_end) {
+        fetch(page, kb + kHop, 0, k_a);
+        page = page_of(kb + 2 * kHop);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      use(kb, 1, k_b);
+      kb += kHop;
+      if (kb >= k_end) break;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+  };
+
   // ---- the stages -------------------------------------------------------------------------------------------------------
   // At the top of stage s its keys are in buffer s & 1 for everybody and stage s + 1 is on its way into the other buffer.
-  if (n_stages > 0) {
+  if (own_blocks) {
+    __syncthreads();  // the flag is cleared
+    if constexpr (kOwnBlocks) few_rows();
+  } else if (n_stages > 0) {
     __syncthreads();  // the flag is cleared
     stage_arrived(k0, 0);
     lds_barrier();
