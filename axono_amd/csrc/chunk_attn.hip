@@ -59,34 +59,41 @@ struct Cfg {
   static constexpr int UPR = D / E;                                    // units per row
   static constexpr int SW = (UPR < 16 ? UPR : 16) - 1;                 // swizzle mask
   static constexpr int VEC = KS * UPR / kThreads;                      // units per thread, tensor and stage
+  static constexpr bool kOwnBlocks = sizeof(T) == 2 && D <= 128;       // see Wave::own_blocks
   static constexpr int STATE = D + 4;                                  // row stride of the states added up in LDS
   static constexpr int kStageBytes = 4 * KS * D * static_cast<int>(sizeof(T));
   // wavefronts with keys of their own in a tile of few rows
-  static constexpr int kDealt = sizeof(T) == 2 && D <= 128 ? kWavesWg : (KS / kBlockKeys < kWavesWg ? KS / kBlockKeys : kWavesWg);
+  static constexpr int kDealt = kOwnBlocks ? kWavesWg : (KS / kBlockKeys < kWavesWg ? KS / kBlockKeys : kWavesWg);
   static constexpr int kStateBytes = kDealt * FEW * (STATE + 2) * 4;
   static constexpr int kLdsBytes = (kStageBytes > kStateBytes ? kStageBytes : kStateBytes) + 16;
 };
 
 // ---- the cut -------------------------------------------------------------------------------------------------------
 struct Seq {
-  int c0, rows, tiles, units, pieces;  // first token, rows per kv head, tiles, 128-key units of the last tile, pieces a tile
+  int c0, start, rows, tiles;  // first token, its position, rows per kv head, tiles
+  int units;                   // of 128 keys, of the last tile
 };
 template <int TR>
 __device__ __forceinline__ Seq load_seq(const ChunkArgs &a, int b) {
-  Seq s{0, 0, 0, 0, 1};
+  Seq s{0, 0, 0, 0, 0};
   if (b < a.B) {
     s.c0 = min(max(a.cu[b], 0), a.tokens);
     const int c1 = min(max(a.cu[b + 1], s.c0), a.tokens);
     const int n = min(c1 - s.c0, a.max_q);
-    const int64_t last = static_cast<int64_t>(a.start[b]) + n;  // keys the last token sees
-    const int keys = static_cast<int>(last < 0 ? 0 : (last > a.max_len ? a.max_len : last));
+    s.start = a.start[b];
+    const int64_t last = static_cast<int64_t>(s.start) + n;  // keys the last token sees
+    s.units = (static_cast<int>(last < 0 ? 0 : (last > a.max_len ? a.max_len : last)) + 127) >> 7;
     s.rows = n * a.group;
     s.tiles = (s.rows + TR - 1) / TR;
-    s.units = (keys + 127) >> 7;
   }
   return s;
 }
-// Units per piece: the work of the launch (every tile taken as long as its sequence's last) over the pieces aimed at.
+// The last key that row r of a sequence sees, -1: none.
+__device__ __forceinline__ int last_key(const ChunkArgs &a, int start, int r) {
+  const int64_t p = static_cast<int64_t>(start) + r / a.group;
+  return static_cast<int>(p < -1 ? -1 : (p > a.max_len - 1 ? a.max_len - 1 : p));
+}
+// Units per piece: the work of a kv head (every tile taken as long as its sequence's last) over the pieces aimed at.
 template <int TR>
 __device__ __forceinline__ int units_per_piece(const ChunkArgs &a, int lane) {
   float work = 0.f;
@@ -95,29 +102,32 @@ __device__ __forceinline__ int units_per_piece(const ChunkArgs &a, int lane) {
     work += group_sum<64>(static_cast<float>(s.tiles) * static_cast<float>(s.units));
   }
   const float q = ceilf(work * static_cast<float>(a.Hkv) / static_cast<float>(a.target));
-  return max(kMinPieceUnits, static_cast<int>(fminf(q, 1.0e9f)));
+  return __builtin_amdgcn_readfirstlane(max(kMinPieceUnits, static_cast<int>(fminf(q, 1.0e9f))));
 }
-__device__ __forceinline__ int pieces_of(int units, int per) { return max(1, (units + per - 1) / per); }
+// Pieces of every tile of a sequence.  One that has few rows only streams keys, each its own: shorter pieces spread such
+// streams better over the device, while tiles of many rows that start together share their keys in the caches.
+template <int FEW>
+__device__ __forceinline__ int pieces_of(const Seq &s, int per) {
+  const int p = s.rows <= FEW ? max(kMinPieceUnits, (per + 1) / 2) : per;
+  return max(1, (s.units + p - 1) / p);
+}
 
 struct Piece {
-  int b, tile, piece, pieces, slot, c0, rows, units;
-  bool found;
+  int b, tile, piece, pieces, slot, c0, start, rows;
 };
-// The `flat`-th piece (MERGE: the `flat`-th cut tile) of the launch, per kv head.  slot: number of the piece (MERGE: of the
-// tile's first piece) among the pieces of cut tiles.
-template <int TR, bool MERGE>
-__device__ __forceinline__ Piece find_piece(const ChunkArgs &a, int flat, int lane) {
+// The `flat`-th piece (MERGE: the `flat`-th cut tile) of a kv head; false: there is none.  slot: number of the piece (MERGE: of
+// the tile's first piece) among the pieces of cut tiles.
+template <int TR, int FEW, bool MERGE>
+__device__ __forceinline__ bool find_piece(const ChunkArgs &a, int flat, int lane, Piece &p) {
   const int per = units_per_piece<TR>(a, lane);
   int done = 0, slots = 0;
-  Piece p{};
-  p.found = false;
   for (int j = 0; j < a.B; j += 64) {
-    Seq s = load_seq<TR>(a, j + lane);
-    s.pieces = pieces_of(s.units, per);
-    const bool cut = s.pieces > 1;
-    const int mine = MERGE ? (cut ? s.tiles : 0) : s.tiles * s.pieces;
+    const Seq s = load_seq<TR>(a, j + lane);
+    const int pieces = pieces_of<FEW>(s, per);
+    const bool cut = pieces > 1;
+    const int mine = MERGE ? (cut ? s.tiles : 0) : s.tiles * pieces;
     const int upto = done + wave_prefix_i32(mine);
-    const int my_slots = cut ? s.tiles * s.pieces : 0;
+    const int my_slots = cut ? s.tiles * pieces : 0;
     const int slots_upto = slots + wave_prefix_i32(my_slots);
     const uint64_t hit = __ballot(flat < upto);
     if (hit) {
@@ -126,21 +136,19 @@ __device__ __forceinline__ Piece find_piece(const ChunkArgs &a, int flat, int la
       const int rest = flat - at(upto - mine);
       p.b = j + l;
       p.c0 = at(s.c0);
+      p.start = at(s.start);
       p.rows = at(s.rows);
-      p.units = at(s.units);
-      p.pieces = at(s.pieces);
-      const int tiles = at(s.tiles);
+      p.pieces = at(pieces);
       const int order = MERGE ? rest : rest / p.pieces;
       p.piece = MERGE ? 0 : rest - order * p.pieces;
-      p.tile = tiles - 1 - order;  // the tiles that see most keys first
+      p.tile = at(s.tiles) - 1 - order;  // the tiles that see most keys first
       p.slot = at(slots_upto - my_slots) + p.tile * p.pieces + p.piece;
-      p.found = true;
-      return p;
+      return true;
     }
     done = __builtin_amdgcn_readlane(upto, 63);
     slots = __builtin_amdgcn_readlane(slots_upto, 63);
   }
-  return p;
+  return false;
 }
 
 // ---- LDS reads of the products' operands -----------------------------------------------------------------------------
@@ -199,77 +207,105 @@ __device__ __forceinline__ float add_weighted(float sum, float w, float o) {
 
 extern __shared__ __attribute__((aligned(16))) unsigned char chunk_smem[];
 
+// One wavefront's part of a piece of a tile: its rows' queries, statistics and results, and the steps of a block of 32 keys.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 1)) void chunk_attn_kernel(ChunkArgs a) {
+struct Wave {
   using C = Cfg<T, D>;
-  using S = typename std::conditional<sizeof(T) == 2, _Float16, float>::type;
-  constexpr int NT = C::NT, KS = C::KS, UPR = C::UPR, VEC = C::VEC, SW = C::SW;
-  constexpr int DT = D / 16;
-  constexpr int QF = sizeof(T) == 2 ? D / 32 : D / 4;  // operand registers of a column tile (8 halves or 1 float each)
-  constexpr bool kHalf = sizeof(T) == 2;
-  constexpr int kRow = D * static_cast<int>(sizeof(T)), kTensor = 2 * KS * kRow;  // bytes: a row, both stages of K (V behind)
-  lds_byte *smem = (lds_byte *)chunk_smem;
-  int *s_flag = reinterpret_cast<int *>(chunk_smem + C::kLdsBytes - 16);
+  static constexpr bool kHalf = sizeof(T) == 2;
+  using S = typename std::conditional<kHalf, _Float16, float>::type;
+  using KFrag = typename std::conditional<kHalf, half8_t, float>::type;
+  using Probs = typename std::conditional<kHalf, half8_t, float8_t>::type;
+  static constexpr int NT = C::NT, KS = C::KS, UPR = C::UPR, SW = C::SW, DT = D / 16;
+  static constexpr int QF = kHalf ? D / 32 : D / 4;  // operand registers of a column tile (8 halves or 1 float each)
+  static constexpr int kRow = D * static_cast<int>(sizeof(T)), kTensor = 2 * KS * kRow;  // bytes: a row, both stages of K
 
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int c = lane & 15, g = lane >> 4;
-  const int hk = blockIdx.x % a.Hkv;
-  const Piece pc = find_piece<C::TR, false>(a, blockIdx.x / a.Hkv, lane);
-  if (!pc.found) return;
-  const int start = a.start[pc.b];
-  const int row0 = pc.tile * C::TR, n_rows = min(pc.rows - row0, C::TR);
-  const bool few = n_rows <= C::FEW;
-  if (tid == 0) *s_flag = 0;
-
-  // this wavefront's rows (positions never fall with the row); rows past the tile repeat its last one and are not stored
-  auto position = [&](int r) {  // last key row r of the tile sees, -1: none
-    const int64_t p = static_cast<int64_t>(start) + (row0 + r) / a.group;
-    return static_cast<int>(p < -1 ? -1 : (p > a.max_len - 1 ? a.max_len - 1 : p));
-  };
-  const int wrow = few ? 0 : wave * 16 * NT;
-  int pos[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) pos[t] = position(min(wrow + t * 16 + c, n_rows - 1));
-  const int wave_first = position(min(wrow, n_rows - 1)), wave_last = position(min(wrow + 16 * NT, n_rows) - 1);
-  const bool idle = wrow >= n_rows;  // a wavefront without rows only loads
-  const int tile_first = position(0), k_all = position(n_rows - 1) + 1;  // keys the tile sees: [0, k_all)
-  const int tile_units = (k_all + 127) >> 7;
-  const int k0 = static_cast<int>(static_cast<int64_t>(tile_units) * pc.piece / pc.pieces) << 7;
-  const int k_end = min(static_cast<int>(static_cast<int64_t>(tile_units) * (pc.piece + 1) / pc.pieces) << 7, k_all);
-  const int n_stages = k_end > k0 ? (k_end - k0 + KS - 1) / KS : 0;
-  // V rows past the tile's last key are stored as zeros, and in stages that some row of the tile must not see whole,
-  // infinities and NaN of V are stored as zeros too (0 * inf is NaN) and added at the end to the rows that see them
-  const int mixed_from = tile_first < 0 ? 0 : (tile_first + 1) / KS * KS;
-
-  // K and V go from memory to LDS directly (16 bytes a lane; a wavefront fills 1 KiB in lane order, so the swizzle is made on
-  // the side of memory: the lane of place u of a row fetches unit u ^ (row & SW)).  Load p of a thread covers row
-  // p kStep + tid / UPR of the stage; its offset within the page differs by constants from load 0's.
-  constexpr int kStep = kThreads / UPR;
-  const unsigned voff = tid / UPR * kRow + ((tid % UPR) ^ ((tid / UPR) & SW)) * 16;
-  // Where this lane reads its operands, as byte offsets into a stage of K / V; the steps of the products flip or add constant
-  // bits of them.  Made opaque in every block, or the compiler keeps every one of the flipped offsets in registers.
-  const int kaddr = c * kRow + (kHalf ? (g ^ (c & SW)) * 16 : (c & SW) * 16 + g * 4);
-  const int vkey = kHalf ? 4 * g + (c >> 2) : 4 * g;
-  const int vaddr = vkey * kRow + (kHalf ? ((((c & 3) >> 1) ^ (vkey & SW)) * 16 + (c & 1) * 8) : (((c >> 2) ^ (vkey & SW)) * 16 + (c & 3) * 4));
+  const ChunkArgs &a;
+  const Piece &pc;
+  int tid, wave, lane, c, g, hk;
+  int row0, n_rows, wrow;            // the tile's first row, its rows, this wavefront's first
+  int k0, k_end, mixed_from;         // keys of the piece; see clean()
+  int wave_first, wave_last;         // last keys that the first and the last of the wavefront's rows see
+  int pos[NT];                       // of this lane's rows
+  int kaddr, vaddr;
+  const T *kbase, *vbase;
+  int64_t page_elems;
   // page numbers by scalar loads: a vector load would have to be waited for behind the stage on its way
   typedef const int32_t __attribute__((address_space(4))) *scalar_ptr;
-  const scalar_ptr table = (scalar_ptr)(a.page_table + static_cast<int64_t>(pc.b) * a.max_pages);
-  const int64_t page_elems = static_cast<int64_t>(a.Hkv) * kPageKeys * D;
-  const T *kbase = static_cast<const T *>(a.k) + static_cast<int64_t>(hk) * kPageKeys * D;
-  const T *vbase = static_cast<const T *>(a.v) + static_cast<int64_t>(hk) * kPageKeys * D;
-  auto in_pool = [&](int page) { return min(max(page, 0), a.n_pages - 1); };
-  auto load_stage = [&](int page, int key0, int buf) __attribute__((always_inline)) {
-    const int64_t base = in_pool(page) * page_elems + static_cast<int64_t>(key0 & (kPageKeys - 1)) * D;
-    const unsigned place = buf * (KS * kRow) + wave * 1024;
+  scalar_ptr table;
+  lds_byte *smem;
+  int *flag;                         // some unit of V was cleaned
+  KFrag qf[NT][QF];
+  float4_t o[NT][DT], lsum[NT];
+  float m[NT];
+
+  __device__ __forceinline__ Wave(const ChunkArgs &args, const Piece &piece, int head, bool few)
+      : a(args), pc(piece), hk(head) {
+    tid = threadIdx.x;
+    wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    lane = tid & 63;
+    c = lane & 15;
+    g = lane >> 4;
+    smem = (lds_byte *)chunk_smem;
+    flag = reinterpret_cast<int *>(chunk_smem + C::kLdsBytes - 16);
+    row0 = pc.tile * C::TR;
+    n_rows = min(pc.rows - row0, C::TR);
+    // rows past the tile repeat its last one and are not stored
+    wrow = few ? 0 : wave * 16 * NT;
 #pragma unroll
-    for (int p = 0; p < VEC; ++p) {
-      const unsigned off = (voff ^ ((p * kStep & SW) * 16)) + p * kStep * kRow;
-      load_lds16(kbase + base, off, smem + place + p * kThreads * 16);
-      load_lds16(vbase + base, off, smem + kTensor + place + p * kThreads * 16);
+    for (int t = 0; t < NT; ++t) pos[t] = position(min(wrow + t * 16 + c, n_rows - 1));
+    wave_first = position(min(wrow, n_rows - 1));
+    wave_last = position(min(wrow + 16 * NT, n_rows) - 1);
+    const int tile_first = position(0), k_all = position(n_rows - 1) + 1;  // keys the tile sees: [0, k_all)
+    const int units = (k_all + 127) >> 7;
+    k0 = static_cast<int>(static_cast<int64_t>(units) * pc.piece / pc.pieces) << 7;
+    k_end = min(static_cast<int>(static_cast<int64_t>(units) * (pc.piece + 1) / pc.pieces) << 7, k_all);
+    mixed_from = tile_first < 0 ? 0 : (tile_first + 1) / KS * KS;
+    table = (scalar_ptr)(a.page_table + static_cast<int64_t>(pc.b) * a.max_pages);
+    page_elems = static_cast<int64_t>(a.Hkv) * kPageKeys * D;
+    kbase = static_cast<const T *>(a.k) + static_cast<int64_t>(hk) * kPageKeys * D;
+    vbase = static_cast<const T *>(a.v) + static_cast<int64_t>(hk) * kPageKeys * D;
+    // Where this lane reads its operands, as byte offsets into a stage of K / V; the steps of the products flip or add constant
+    // bits of them.  Made opaque where they are used, or the compiler keeps every one of the flipped offsets in registers.
+    kaddr = c * kRow + (kHalf ? (g ^ (c & SW)) * 16 : (c & SW) * 16 + g * 4);
+    const int vkey = kHalf ? 4 * g + (c >> 2) : 4 * g;
+    vaddr = vkey * kRow + (kHalf ? ((((c & 3) >> 1) ^ (vkey & SW)) * 16 + (c & 1) * 8) : (((c >> 2) ^ (vkey & SW)) * 16 + (c & 3) * 4));
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      m[t] = kMasked;
+      lsum[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[t][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-  };
-  // V of key `key` in LDS: zeros behind the piece, no infinities and NaN; whether there were any.
-  auto clean_unit = [&](lds_byte *place, int key) __attribute__((always_inline)) {
+  }
+
+  __device__ __forceinline__ int position(int r) const { return last_key(a, pc.start, row0 + r); }
+  __device__ __forceinline__ int64_t row_at(int r) const {  // of q and out
+    const int rr = row0 + r, i = rr / a.group;
+    return (static_cast<int64_t>(pc.c0 + i) * a.Hq + hk * a.group + (rr - i * a.group)) * D;
+  }
+  __device__ __forceinline__ int page_of(int key) const { return table[min(key, k_end - 1) >> kPageShift]; }
+  __device__ __forceinline__ int64_t key_at(int page, int key) const {  // a page number outside the pool is clamped into it
+    return min(max(page, 0), a.n_pages - 1) * page_elems + static_cast<int64_t>(key & (kPageKeys - 1)) * D;
+  }
+
+  // Q as the right operand of the first product, for the whole piece
+  __device__ __forceinline__ void load_q() {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const S *qrow = static_cast<const S *>(a.q) + row_at(min(wrow + t * 16 + c, n_rows - 1));
+#pragma unroll
+      for (int kk = 0; kk < QF; ++kk) {
+        if constexpr (kHalf) qf[t][kk] = *reinterpret_cast<const half8_t *>(qrow + kk * 32 + g * 8);
+        else qf[t][kk] = qrow[kk * 4 + g];
+      }
+    }
+  }
+
+  // Zero probability times infinity or NaN is NaN, so V must not hold any where some row of the tile does not see its key.
+  // clean(): a 16-byte unit of V of key `key` in LDS becomes zeros behind the piece's last key, and loses its infinities and
+  // NaN (true: it had some); finish() gives them at the end to the rows that see them.  Keys from mixed_from on, a multiple
+  // of KS, are cleaned: every key that some row does not see is among them, and every key behind the last.
+  __device__ __forceinline__ bool clean(lds_byte *place, int key) const {
     typedef u32x4_t __attribute__((address_space(3))) lds_unit;
     lds_unit *at = reinterpret_cast<lds_unit *>(place);
     const u32x4_t u = *at;
@@ -280,59 +316,27 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
       return true;
     }
     return false;
-  };
-  // The units that this thread has fetched are in LDS.  (In its own order: the barrier behind this call makes them everybody's.)
-  auto stage_arrived = [&](int key0, int buf) __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (key0 + KS > mixed_from) {  // uniform; also every stage that reaches past k_end, for mixed_from <= k_all
-      bool bad = false;
-#pragma unroll 1
-      for (int p = 0; p < VEC; ++p)
-        bad |= clean_unit(smem + kTensor + buf * (KS * kRow) + (p * kThreads + tid) * 16, key0 + p * kStep + tid / UPR);
-      if (bad) *s_flag = 1;
-    }
-  };
-
-  const bool own_blocks = few && kHalf && D <= 128;
-  if (n_stages > 0 && !own_blocks) load_stage(table[k0 >> kPageShift], k0, 0);
-
-  // Q as the right operand of the first product, for the whole kernel
-  typename std::conditional<kHalf, half8_t, float>::type qf[NT][QF];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int r = row0 + min(wrow + t * 16 + c, n_rows - 1), i = r / a.group;
-    const S *qrow = static_cast<const S *>(a.q) +
-                    (static_cast<int64_t>(pc.c0 + i) * a.Hq + hk * a.group + (r - i * a.group)) * D;
-#pragma unroll
-    for (int kk = 0; kk < QF; ++kk) {
-      if constexpr (kHalf) qf[t][kk] = *reinterpret_cast<const half8_t *>(qrow + kk * 32 + g * 8);
-      else qf[t][kk] = qrow[kk * 4 + g];
-    }
   }
 
-  float4_t o[NT][DT], lsum[NT];
-  float m[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    m[t] = kMasked;
-    lsum[t] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[t][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
-  }
-
-  // ---- a block of 32 keys for this wavefront, in four parts ------------------------------------------------------------
-  using KFrag = typename std::conditional<kHalf, half8_t, float>::type;
-  using Probs = typename std::conditional<kHalf, half8_t, float8_t>::type;
-  auto read_k = [&](int buf, int sub, KFrag (&kf)[2][QF]) __attribute__((always_inline)) {
-    const lds_byte *k_l = smem + sub * (kBlockKeys * kRow);
-    int ka = kaddr + buf * (KS * kRow);
+  __device__ __forceinline__ void read_k(int place, KFrag (&kf)[2][QF]) const {  // place: byte offset of the block's rows
+    int ka = kaddr + place;
     asm volatile("" : "+v"(ka));
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk)
 #pragma unroll
-      for (int kk = 0; kk < QF; ++kk) kf[tk][kk] = lds_at<KFrag>(k_l, (ka ^ (kk * (kHalf ? 64 : 16))) + tk * 16 * kRow);
-  };
-  auto scores = [&](const KFrag (&kf)[2][QF], float4_t (&sc)[NT][2]) __attribute__((always_inline)) {
+      for (int kk = 0; kk < QF; ++kk) kf[tk][kk] = lds_at<KFrag>(smem, (ka ^ (kk * (kHalf ? 64 : 16))) + tk * 16 * kRow);
+  }
+  // fp16: V^T fragments of a block, d tile by d tile
+  __device__ __forceinline__ void read_v(int place, half8_t (&vf)[DT]) const {
+    int va = vaddr + place;
+    asm volatile("" : "+v"(va));
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const half4_t lo = lds_tr(smem, va ^ (dt * 32)), hi = lds_tr(smem, (va ^ (dt * 32)) + 16 * kRow);
+      vf[dt] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  __device__ __forceinline__ void scores(const KFrag (&kf)[2][QF], float4_t (&sc)[NT][2]) const {
 #pragma unroll
     for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -344,30 +348,31 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
           if constexpr (kHalf) sc[t][tk] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tk][kk], qf[t][kk], sc[t][tk], 0, 0, 0);
           else sc[t][tk] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[tk][kk], qf[t][kk], sc[t][tk], 0, 0, 0);
         }
-  };
+  }
+  template <bool MASK>
+  __device__ __forceinline__ float score(const float4_t (&sc)[NT][2], int kb, int t, int j) const {
+    const float v = sc[t][j >> 2][j & 3];
+    return MASK && kb + (j >> 2) * 16 + 4 * g + (j & 3) > pos[t] ? kMasked : v;
+  }
+  template <bool MASK>
+  __device__ __forceinline__ void exps(const float4_t (&sc)[NT][2], int kb, float (&p)[NT][8]) const {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = score<MASK>(sc, kb, t, j);
+        p[t][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.scale_log2e, -m[t]));
+        if (MASK && x <= kMasked) p[t][j] = 0.f;
+      }
+  }
   // Probabilities against the running maximum as it stands: it is moved, and everything rescaled, only when one of them
   // passes 2^8 (the first block of a row always does).  Until then p <= 256, which fp16 holds to the same 11 bits, and a
   // block needs no maximum over its row at all.  (The maximum never runs ahead, so no p is smaller than against the true one.)
   // MASK: some key of the block at kb is behind some row's position.
-  auto softmax = [&](const float4_t (&sc)[NT][2], Probs (&pf)[NT], int kb, auto mask_c) __attribute__((always_inline)) {
-    constexpr bool MASK = decltype(mask_c)::value;
+  template <bool MASK>
+  __device__ __forceinline__ void softmax(const float4_t (&sc)[NT][2], int kb, Probs (&pf)[NT]) {
     float p[NT][8];
-    auto x_at = [&](int t, int j) __attribute__((always_inline)) {
-      float v = sc[t][j >> 2][j & 3];
-      if (MASK && kb + (j >> 2) * 16 + 4 * g + (j & 3) > pos[t]) v = kMasked;
-      return v;
-    };
-    auto exps = [&]() __attribute__((always_inline)) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float x = x_at(t, j);
-          p[t][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, a.scale_log2e, -m[t]));
-          if (MASK && x <= kMasked) p[t][j] = 0.f;
-        }
-    };
-    exps();
+    exps<MASK>(sc, kb, p);
     float top = 0.f;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -376,9 +381,9 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
     if (__builtin_expect(__any(top > 256.f), 0)) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        float mx = x_at(t, 0);
+        float mx = score<MASK>(sc, kb, t, 0);
 #pragma unroll
-        for (int j = 1; j < 8; ++j) mx = fmaxf(mx, x_at(t, j));
+        for (int j = 1; j < 8; ++j) mx = fmaxf(mx, score<MASK>(sc, kb, t, j));
         const float mnew = fmaxf(m[t], max_xor32(max_xor16(mx)) * a.scale_log2e);
         const float corr = __builtin_amdgcn_exp2f(m[t] - mnew);
         m[t] = mnew;
@@ -386,7 +391,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[t][dt] *= corr;
       }
-      exps();
+      exps<MASK>(sc, kb, p);
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -395,19 +400,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
         if constexpr (kHalf) pf[t][j] = static_cast<_Float16>(p[t][j]);
         else pf[t][j] = p[t][j];
       }
-  };
-  // fp16: V^T fragments of the block, d tile by d tile
-  auto read_v = [&](int buf, int sub, half8_t (&vf)[DT]) __attribute__((always_inline)) {
-    const lds_byte *v_l = smem + sub * (kBlockKeys * kRow) + kTensor;
-    int va = vaddr + buf * (KS * kRow);
-    asm volatile("" : "+v"(va));
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const half4_t lo = lds_tr(v_l, va ^ (dt * 32)), hi = lds_tr(v_l, (va ^ (dt * 32)) + 16 * kRow);
-      vf[dt] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-  };
-  auto add_values = [&](const half8_t (&vf)[DT], const Probs (&pf)[NT]) __attribute__((always_inline)) {
+  }
+  __device__ __forceinline__ void add_values(const half8_t (&vf)[DT], const Probs (&pf)[NT]) {
     if constexpr (kHalf) {
       const half8_t ones = {1, 1, 1, 1, 1, 1, 1, 1};
       // the row sums as a product with ones: every register of the result holds the row's sum
@@ -418,12 +412,11 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
 #pragma unroll
         for (int t = 0; t < NT; ++t) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[dt], pf[t], o[t][dt], 0, 0, 0);
     }
-  };
+  }
   // fp32: product step (tk, e) takes keys tk * 16 + 4 g + e, g = 0 .. 3, so that a lane's score register e is its right operand
-  auto add_values_f32 = [&](int buf, int sub, const Probs (&pf)[NT]) __attribute__((always_inline)) {
+  __device__ __forceinline__ void add_values_f32(int place, const Probs (&pf)[NT]) {
     if constexpr (!kHalf) {
-      const lds_byte *v_l = smem + sub * (kBlockKeys * kRow) + kTensor;
-      int va = vaddr + buf * (KS * kRow);
+      int va = vaddr + place;
       asm volatile("" : "+v"(va));
 #pragma unroll
       for (int tk = 0; tk < 2; ++tk)
@@ -433,158 +426,107 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
           for (int t = 0; t < NT; ++t) lsum[t][0] += pf[t][tk * 4 + e];
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
-            const float vf = lds_at<float>(v_l, (va ^ (dt * 64) ^ (e * 16)) + (tk * 16 + e) * kRow);
+            const float vf = lds_at<float>(smem, (va ^ (dt * 64) ^ (e * 16)) + (tk * 16 + e) * kRow);
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, pf[t][tk * 4 + e], o[t][dt], 0, 0, 0);
           }
         }
     }
-  };
-  auto block = [&](int buf, int sub, int kb, auto mask_c) __attribute__((always_inline)) {
+  }
+  template <bool MASK>
+  __device__ __forceinline__ void block(int buf, int sub, int kb) {
     KFrag kf[2][QF];
     float4_t sc[NT][2];
     Probs pf[NT];
-    read_k(buf, sub, kf);
+    const int place = (buf * KS + sub * kBlockKeys) * kRow;
+    read_k(place, kf);
     scores(kf, sc);
-    softmax(sc, pf, kb, mask_c);
+    softmax<MASK>(sc, kb, pf);
     if constexpr (kHalf) {
       half8_t vf[DT];
-      read_v(buf, sub, vf);
+      read_v(kTensor + place, vf);
       add_values(vf, pf);
     } else {
-      add_values_f32(buf, sub, pf);
+      add_values_f32(kTensor + place, pf);
     }
-  };
+  }
 
-  // ---- a tile with few rows, fp16 ------------------------------------------------------------------------------------------
-  // Bound by the stream of keys, so every wavefront takes blocks of its own (block i of the piece goes to wavefront i % 4) and
-  // waits for nobody: K goes to registers in operand order (16 rows x 64 bytes a load), V through a strip of LDS of the
-  // wavefront's own, both a block ahead, read once and therefore past the caches.
-  constexpr bool kOwnBlocks = kHalf && D <= 128;
-  auto few_rows = [&]() __attribute__((always_inline)) {
-    constexpr int kVBytes = kBlockKeys * kRow, kLoads = kVBytes / 1024;  // V of a block; loads of a lane for it, as many for K
-    constexpr int kRowsALoad = 1024 / kRow;
-    static_assert(!kOwnBlocks || 2 * kWavesWg * kVBytes <= C::kStageBytes, "two blocks of V per wavefront fit the stages' LDS");
-    auto fetch = [&](int page, int kb, int buf, KFrag (&kf)[2][QF]) __attribute__((always_inline)) {
-      const int64_t base = in_pool(page) * page_elems + static_cast<int64_t>(kb & (kPageKeys - 1)) * D;
-      int l = lane;
-      asm volatile("" : "+v"(l));  // offsets are made here, not kept
-      const unsigned v_row = static_cast<unsigned>(l) / UPR, v_off = v_row * kRow + ((l % UPR) ^ (v_row & SW)) * 16;
+  // ---- the keys in stages that the workgroup shares -------------------------------------------------------------------------
+  // K and V go from memory to LDS directly (16 bytes a lane; a wavefront fills 1 KiB in lane order, so the swizzle is made on
+  // the side of memory: the lane of place u of a row fetches unit u ^ (row & SW)).  Load p of a thread covers row
+  // p kStep + tid / UPR of the stage; its offset within the page differs by constants from load 0's.
+  static constexpr int kStep = kThreads / UPR;
+  __device__ __forceinline__ void load_stage(int page, int key0, int buf) const {
+    const int64_t base = key_at(page, key0);
+    const unsigned place = buf * (KS * kRow) + wave * 1024;
+    const unsigned voff = tid / UPR * kRow + ((tid % UPR) ^ ((tid / UPR) & SW)) * 16;
 #pragma unroll
-      for (int p = 0; p < kLoads; ++p)
-        load_lds16<T, 2>(vbase + base, (v_off ^ ((p * kRowsALoad & SW) * 16)) + p * 1024, smem + (wave * 2 + buf) * kVBytes + p * 1024);
-      const T *kb_ = kbase + base + (l & 15) * D + (l >> 4) * 8;
-#pragma unroll
-      for (int tk = 0; tk < 2; ++tk)
-#pragma unroll
-        for (int kk = 0; kk < QF; ++kk)
-          if constexpr (kHalf)
-            kf[tk][kk] = __builtin_bit_cast(half8_t, __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(kb_ + tk * 16 * D + kk * 32)));
-    };
-    auto use = [&](int kb, int buf, const KFrag (&kf)[2][QF]) __attribute__((always_inline)) {
-      float4_t sc[NT][2];
-      Probs pf[NT];
-      scores(kf, sc);
-      __builtin_amdgcn_sched_barrier(0);
-      if (kb + kBlockKeys > mixed_from) {
+    for (int p = 0; p < C::VEC; ++p) {
+      const unsigned off = (voff ^ ((p * kStep & SW) * 16)) + p * kStep * kRow;
+      load_lds16(kbase + base, off, smem + place + p * kThreads * 16);
+      load_lds16(vbase + base, off, smem + kTensor + place + p * kThreads * 16);
+    }
+  }
+  // The units that this thread has fetched are in LDS, and clean.  (The barrier behind this call makes them everybody's.)
+  __device__ __forceinline__ void stage_arrived(int key0, int buf) const {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (key0 + KS > mixed_from) {  // uniform
+      bool bad = false;
 #pragma unroll 1
-        for (int p = 0; p < kLoads; ++p)
-          if (clean_unit(smem + (wave * 2 + buf) * kVBytes + p * 1024 + lane * 16, kb + static_cast<int>(lane / UPR) + p * kRowsALoad)) *s_flag = 1;
-      }
-      softmax(sc, pf, kb, std::true_type{});
-      __builtin_amdgcn_sched_barrier(0);
-      half8_t vf[DT];
-      int va = vaddr + (wave * 2 + buf) * kVBytes;
-      asm volatile("" : "+v"(va));
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const half4_t lo = lds_tr(smem, va ^ (dt * 32)), hi = lds_tr(smem, (va ^ (dt * 32)) + 16 * kRow);
-        vf[dt] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      }
-      add_values(vf, pf);
-    };
-    constexpr int kHop = kWavesWg * kBlockKeys;  // 128 keys: the wavefront's next block lies in the next page
-    KFrag k_a[2][QF], k_b[2][QF];
-    int kb = k0 + wave * kBlockKeys;
-    if (kb >= k_end) return;
-    auto page_of = [&](int key) { return table[min(key, k_end - 1) >> kPageShift]; };
-    fetch(page_of(kb), kb, 0, k_a);
-    int page = page_of(kb + kHop);
-    // the loads of the block in use have arrived when no more than the next block's are under way (loads return in order)
-    while (true) {
-      if (kb + kHop < k_end) {
-        fetch(page, kb + kHop, 1, k_b);
-        page = page_of(kb + 2 * kHop);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
-      } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      }
-      use(kb, 0, k_a);
-      kb += kHop;
-      if (kb >= k_end) break;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V of the block just used is in registers: its strip is free
-      if (kb + kHop < k_end) {
-        fetch(page, kb + kHop, 0, k_a);
-        page = page_of(kb + 2 * kHop);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
-      } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      }
-      use(kb, 1, k_b);
-      kb += kHop;
-      if (kb >= k_end) break;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      for (int p = 0; p < C::VEC; ++p)
+        bad |= clean(smem + kTensor + buf * (KS * kRow) + (p * kThreads + tid) * 16, key0 + p * kStep + tid / UPR);
+      if (bad) *flag = 1;
     }
-  };
-
-  // ---- the stages -------------------------------------------------------------------------------------------------------
+  }
   // At the top of stage s its keys are in buffer s & 1 for everybody and stage s + 1 is on its way into the other buffer.
-  if (own_blocks) {
+  // few: the wavefronts have the same rows and deal the blocks of a stage.
+  __device__ __forceinline__ void shared_stages(bool few) {
+    const int n_stages = k_end > k0 ? (k_end - k0 + KS - 1) / KS : 0;
+    const bool idle = wrow >= n_rows;  // a wavefront without rows only loads
+    if (n_stages > 0) load_stage(page_of(k0), k0, 0);
+    load_q();
     __syncthreads();  // the flag is cleared
-    if constexpr (kOwnBlocks) few_rows();
-  } else if (n_stages > 0) {
-    __syncthreads();  // the flag is cleared
+    if (n_stages == 0) return;
     stage_arrived(k0, 0);
     lds_barrier();
-    if (n_stages > 1) load_stage(table[(k0 + KS) >> kPageShift], k0 + KS, 1);
-    auto page_after = [&](int s) { return table[min(k0 + (s + 2) * KS, k_end - 1) >> kPageShift]; };
-    int s = 0, page = page_after(0);
+    if (n_stages > 1) load_stage(page_of(k0 + KS), k0 + KS, 1);
+    int s = 0, page = page_of(k0 + 2 * KS);
     // Stages that every row of the tile sees whole run as a software pipeline: while one block's scores and values are
     // multiplied, the next operands come from LDS, so a wavefront never waits for an LDS read that it has just made.  The
     // barrier that ends a stage stands in the middle of its last block, behind that block's last LDS read.
     if constexpr (kHalf && KS == 2 * kBlockKeys) {
-      const int n_fast = few || tile_first < k0 ? 0 : min((tile_first + 1 - k0) / KS, n_stages);
+      const int seen = position(0) + 1 - k0;  // keys of the piece that all rows see
+      const int n_fast = few || seen <= 0 ? 0 : min(seen / KS, n_stages);
       if (n_fast > 0) {
         KFrag kf[2][QF];
-        if (!idle) read_k(0, 0, kf);
+        if (!idle) read_k(0, kf);
         for (; s < n_fast; ++s) {
-          const int buf = s & 1, key0 = k0 + s * KS;
-          const bool more = s + 1 < n_stages;
+          const int buf = s & 1, key0 = k0 + s * KS, place = buf * (KS * kRow);
           half8_t vf[DT];
           float4_t sc[NT][2];
           Probs pf[NT];
           if (!idle) {
             scores(kf, sc);
-            read_v(buf, 0, vf);
-            read_k(buf, 1, kf);
+            read_v(kTensor + place, vf);
+            read_k(place + kBlockKeys * kRow, kf);
             __builtin_amdgcn_sched_barrier(0);
-            softmax(sc, pf, key0, std::false_type{});
+            softmax<false>(sc, key0, pf);
             add_values(vf, pf);
             __builtin_amdgcn_sched_barrier(0);
             scores(kf, sc);
-            read_v(buf, 1, vf);
+            read_v(kTensor + place + kBlockKeys * kRow, vf);
           }
-          if (more) {
+          if (s + 1 < n_stages) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             stage_arrived(key0 + KS, buf ^ 1);
             lds_barrier();
             if (s + 2 < n_stages) load_stage(page, key0 + 2 * KS, buf);
-            page = page_after(s + 1);
+            page = page_of(key0 + 3 * KS);
           }
           __builtin_amdgcn_sched_barrier(0);
           if (!idle) {
-            if (s + 1 < n_fast) read_k(buf ^ 1, 0, kf);
-            softmax(sc, pf, key0, std::false_type{});
+            if (s + 1 < n_fast) read_k((buf ^ 1) * (KS * kRow), kf);
+            softmax<false>(sc, key0, pf);
             add_values(vf, pf);
           }
           __builtin_amdgcn_sched_barrier(0);
@@ -598,69 +540,116 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
         const int kb = key0 + sub * kBlockKeys;
         const bool mine = few ? sub == wave : !idle;
         if (mine && kb <= wave_last && kb < k_end) {  // wave-uniform
-          if (kb + kBlockKeys - 1 > wave_first) block(buf, sub, kb, std::true_type{});
-          else block(buf, sub, kb, std::false_type{});
+          if (kb + kBlockKeys - 1 > wave_first) block<true>(buf, sub, kb);
+          else block<false>(buf, sub, kb);
         }
       }
       if (s + 1 < n_stages) {
         stage_arrived(key0 + KS, buf ^ 1);
         lds_barrier();
         if (s + 2 < n_stages) load_stage(page, key0 + 2 * KS, buf);
-        page = page_after(s + 1);
+        page = page_of(key0 + 3 * KS);
       }
     }
   }
-  if constexpr (!kHalf) {
+
+  // ---- few rows, fp16: every wavefront its own keys ---------------------------------------------------------------------------
+  // Bound by the stream of keys, so every wavefront takes blocks of its own (block i of the piece goes to wavefront i % 4) and
+  // waits for nobody: K goes to registers in operand order (16 rows x 64 bytes a load), V through a strip of LDS of the
+  // wavefront's own, both a block ahead, read once and therefore past the caches.
+  static constexpr int kVBytes = kBlockKeys * kRow, kLoads = kVBytes / 1024;  // V of a block; loads of a lane for it, as many for K
+  __device__ __forceinline__ void fetch_own(int page, int kb, int buf, KFrag (&kf)[2][QF]) const {
+    constexpr int kRowsALoad = 1024 / kRow;
+    static_assert(2 * kWavesWg * kVBytes <= C::kStageBytes, "two blocks of V per wavefront fit the stages' LDS");
+    const int64_t base = key_at(page, kb);
+    int l = lane;
+    asm volatile("" : "+v"(l));  // offsets are made here, not kept
+    const unsigned v_row = static_cast<unsigned>(l) / UPR, v_off = v_row * kRow + ((l % UPR) ^ (v_row & SW)) * 16;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) lsum[t][0] = sum_xor32(sum_xor16(lsum[t][0]));
+    for (int p = 0; p < kLoads; ++p)
+      load_lds16<T, 2>(vbase + base, (v_off ^ ((p * kRowsALoad & SW) * 16)) + p * 1024, smem + (wave * 2 + buf) * kVBytes + p * 1024);
+    const T *rows = kbase + base + (l & 15) * D + (l >> 4) * 8;
+#pragma unroll
+    for (int tk = 0; tk < 2; ++tk)
+#pragma unroll
+      for (int kk = 0; kk < QF; ++kk)
+        kf[tk][kk] = __builtin_bit_cast(half8_t, __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(rows + tk * 16 * D + kk * 32)));
   }
-  __syncthreads();
-  const bool repair = *s_flag != 0;  // uniform
-
-  const bool cut = pc.pieces > 1;
-  const int64_t slot = static_cast<int64_t>(pc.slot) * a.Hkv + hk;
-  if (cut && (slot >= a.slots || n_rows > a.slot_rows)) return;  // (cannot happen: the cut is bounded by both)
-  auto out_row = [&](int r) -> T * {
-    const int rr = row0 + r, i = rr / a.group;
-    return static_cast<T *>(a.out) + (static_cast<int64_t>(pc.c0 + i) * a.Hq + hk * a.group + (rr - i * a.group)) * D;
-  };
-
-  // Infinities and NaN of V that were stored as zeros are added at the end, to element d of every row that sees their key
-  // (a positive weight does not change them): rare, so through memory and without a thought for speed.
-  auto finish = [&]() {
-    if (!repair) return;
-    __threadfence_block();
-    __syncthreads();
-    for (int x = tid; x < n_rows * D; x += kThreads) {
-      const int r = x / D, d = x % D, last = position(r);
-      float sum = 0.f;
-      for (int key = max(k0, mixed_from); key < k_end && key <= last; ++key) {
-        const float v = ldf(vbase + in_pool(table[key >> kPageShift]) * page_elems + static_cast<int64_t>(key & (kPageKeys - 1)) * D + d);
-        if (!(fabsf(v) < __builtin_inff())) sum += v;
-      }
-      if (sum == 0.f) continue;
-      if (cut) a.part_o[(slot * a.slot_rows + r) * D + d] += sum;
-      else stf(out_row(r) + d, ldf(out_row(r) + d) + sum);
+  __device__ __forceinline__ void use_own(int kb, int buf, const KFrag (&kf)[2][QF]) {
+    float4_t sc[NT][2];
+    Probs pf[NT];
+    scores(kf, sc);
+    __builtin_amdgcn_sched_barrier(0);
+    const int strip = (wave * 2 + buf) * kVBytes;
+    if (kb + kBlockKeys > mixed_from) {
+      bool bad = false;
+#pragma unroll 1
+      for (int p = 0; p < kLoads; ++p) bad |= clean(smem + strip + p * 1024 + lane * 16, kb + (p * 64 + lane) / UPR);
+      if (bad) *flag = 1;
     }
-  };
+    softmax<true>(sc, kb, pf);
+    __builtin_amdgcn_sched_barrier(0);
+    half8_t vf[DT];
+    read_v(strip, vf);
+    add_values(vf, pf);
+  }
+  __device__ __forceinline__ void own_blocks() {
+    constexpr int kHop = kWavesWg * kBlockKeys;
+    load_q();
+    __syncthreads();  // the flag is cleared
+    int kb = k0 + wave * kBlockKeys;
+    if (kb >= k_end) return;
+    KFrag now[2][QF], next[2][QF];
+    fetch_own(page_of(kb), kb, 0, now);
+    int page = page_of(kb + kHop);
+#pragma unroll 1
+    for (int buf = 0;; buf ^= 1) {
+      // the block in use has arrived when no more than the next one's loads are under way (loads return in order)
+      if (kb + kHop < k_end) {
+        fetch_own(page, kb + kHop, buf ^ 1, next);
+        page = page_of(kb + 2 * kHop);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      use_own(kb, buf, now);
+      kb += kHop;
+      if (kb >= k_end) break;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V of the block just used is in registers: its strip is free
+#pragma unroll
+      for (int tk = 0; tk < 2; ++tk)
+#pragma unroll
+        for (int kk = 0; kk < QF; ++kk) now[tk][kk] = next[tk][kk];
+    }
+  }
 
-  if (!few) {
+  // ---- the results ----------------------------------------------------------------------------------------------------------
+  __device__ __forceinline__ void sum_lanes() {
+    if constexpr (!kHalf) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) lsum[t][0] = sum_xor32(sum_xor16(lsum[t][0]));
+    }
+  }
+  // no key seen: zeros; a NaN stays one
+  static __device__ __forceinline__ float inverse(float l) { return l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l); }
+  // rows of this wavefront, straight from its registers; `part` >= 0: to that row of the states instead
+  __device__ __forceinline__ void store_rows(int64_t part) {
+    sum_lanes();
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int r = wrow + t * 16 + c;
       if (r >= n_rows) continue;
-      const float l = lsum[t][0];
-      if (cut) {
-        float *po = a.part_o + (slot * a.slot_rows + r) * D;
+      if (part >= 0) {
+        float *po = a.part_o + (part + r) * D;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t *>(po + dt * 16 + 4 * g) = o[t][dt];
         if (g == 0) {
-          a.part_ml[(slot * a.slot_rows + r) * 2] = m[t];
-          a.part_ml[(slot * a.slot_rows + r) * 2 + 1] = l;
+          a.part_ml[(part + r) * 2] = m[t];
+          a.part_ml[(part + r) * 2 + 1] = lsum[t][0];
         }
       } else {
-        const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // no key: zeros; a NaN stays one
-        S *orow = reinterpret_cast<S *>(out_row(r));
+        const float inv = inverse(lsum[t][0]);
+        S *orow = static_cast<S *>(a.out) + row_at(r);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           typedef S vec4 __attribute__((ext_vector_type(4)));
@@ -671,76 +660,149 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
         }
       }
     }
-    finish();
-    return;
   }
+  // the wavefronts have the same rows: their states are added up through LDS (everybody has left it)
+  __device__ __forceinline__ void store_sum(int64_t part) {
+    sum_lanes();
+    float *so = reinterpret_cast<float *>(chunk_smem);
+    float *sml = so + C::kDealt * C::FEW * C::STATE;
+    if (wave < C::kDealt) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int r = wave * C::FEW + t * 16 + c;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t *>(so + r * C::STATE + dt * 16 + 4 * g) = o[t][dt];
+        if (g == 0) {
+          sml[2 * r] = m[t];
+          sml[2 * r + 1] = lsum[t][0];
+        }
+      }
+    }
+    __syncthreads();
+    for (int x = tid; x < n_rows * D; x += kThreads) {
+      const int r = x / D, d = x % D;
+      float mx = kMasked;
+#pragma unroll
+      for (int w = 0; w < C::kDealt; ++w) mx = fmaxf(mx, sml[2 * (w * C::FEW + r)]);
+      float l = 0.f, acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < C::kDealt; ++w) {
+        const float f = __builtin_amdgcn_exp2f(sml[2 * (w * C::FEW + r)] - mx);
+        l = __builtin_fmaf(f, sml[2 * (w * C::FEW + r) + 1], l);
+        acc = add_weighted(acc, f, so[(w * C::FEW + r) * C::STATE + d]);
+      }
+      if (part >= 0) {
+        a.part_o[(part + r) * D + d] = acc;
+        if (d == 0) {
+          a.part_ml[(part + r) * 2] = mx;
+          a.part_ml[(part + r) * 2 + 1] = l;
+        }
+      } else {
+        stf(static_cast<T *>(a.out) + row_at(r) + d, acc * inverse(l));
+      }
+    }
+  }
+  // Infinities and NaN of V that were cleaned away, added to element d of every row that sees their key (a positive weight does
+  // not change them): rare, so through memory and without a thought for speed.
+  __device__ __forceinline__ void finish(bool had, int64_t part) {
+    if (!had) return;
+    __threadfence_block();
+    __syncthreads();
+    for (int x = tid; x < n_rows * D; x += kThreads) {
+      const int r = x / D, d = x % D, last = position(r);
+      float sum = 0.f;
+      for (int key = max(k0, mixed_from); key < k_end && key <= last; ++key) {
+        const float v = ldf(vbase + key_at(table[key >> kPageShift], key) + d);
+        if (!(fabsf(v) < __builtin_inff())) sum += v;
+      }
+      if (sum == 0.f) continue;
+      T *out = static_cast<T *>(a.out) + row_at(r) + d;
+      if (part >= 0) a.part_o[(part + r) * D + d] += sum;
+      else stf(out, ldf(out) + sum);
+    }
+  }
+};
 
-  // few rows: the states of the wavefronts that had keys, through LDS
-  float *so = reinterpret_cast<float *>(chunk_smem);
-  float *sml = so + C::kDealt * C::FEW * C::STATE;
-  if (wave < C::kDealt) {
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int r = wave * C::FEW + t * 16 + c;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t *>(so + r * C::STATE + dt * 16 + 4 * g) = o[t][dt];
-      if (g == 0) {
-        sml[2 * r] = m[t];
-        sml[2 * r + 1] = lsum[t][0];
-      }
-    }
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 1)) void chunk_attn_kernel(ChunkArgs a) {
+  using C = Cfg<T, D>;
+  using W = Wave<T, D>;
+  const int hk = blockIdx.x % a.Hkv;
+  Piece pc;
+  if (!find_piece<C::TR, C::FEW, false>(a, blockIdx.x / a.Hkv, threadIdx.x & 63, pc)) return;
+  const int n_rows = min(pc.rows - pc.tile * C::TR, C::TR);
+  int64_t part = -1;
+  if (pc.pieces > 1) {
+    const int64_t slot = static_cast<int64_t>(pc.slot) * a.Hkv + hk;
+    if (slot >= a.slots || n_rows > a.slot_rows) return;  // (cannot happen: the cut is bounded by both)
+    part = slot * a.slot_rows;
   }
-  __syncthreads();
-  for (int x = tid; x < n_rows * D; x += kThreads) {
-    const int r = x / D, d = x % D;
-    float mx = kMasked;
-#pragma unroll
-    for (int w = 0; w < C::kDealt; ++w) mx = fmaxf(mx, sml[2 * (w * C::FEW + r)]);
-    float l = 0.f, acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < C::kDealt; ++w) {
-      const float f = __builtin_amdgcn_exp2f(sml[2 * (w * C::FEW + r)] - mx);
-      l = __builtin_fmaf(f, sml[2 * (w * C::FEW + r) + 1], l);
-      acc = add_weighted(acc, f, so[(w * C::FEW + r) * C::STATE + d]);
-    }
-    if (cut) {
-      a.part_o[(slot * a.slot_rows + r) * D + d] = acc;
-      if (d == 0) {
-        a.part_ml[(slot * a.slot_rows + r) * 2] = mx;
-        a.part_ml[(slot * a.slot_rows + r) * 2 + 1] = l;
-      }
-    } else {
-      const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-      stf(out_row(r) + d, acc * inv);
-    }
+  int *flag = reinterpret_cast<int *>(chunk_smem + C::kLdsBytes - 16);
+  if (threadIdx.x == 0) *flag = 0;
+  if (n_rows <= C::FEW) {
+    W w(a, pc, hk, true);
+    if constexpr (C::kOwnBlocks) w.own_blocks();
+    else w.shared_stages(true);
+    __syncthreads();
+    const bool had = *flag != 0;
+    w.store_sum(part);
+    w.finish(had, part);
+  } else {
+    W w(a, pc, hk, false);
+    w.shared_stages(false);
+    __syncthreads();
+    const bool had = *flag != 0;
+    w.store_rows(part);
+    w.finish(had, part);
   }
-  finish();
 }
 
-// Adds the pieces of a cut tile: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), in the order of the keys.
+// Adds the pieces of a cut tile: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), in the order of the keys.  A workgroup
+// takes 16 rows; four pieces are on their way at a time.  (Whole tiles per workgroup measured 28 us where this takes 10:
+// few workgroups with a long chain of loads each.)
+constexpr int kMergeRows = 16;
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void chunk_merge_kernel(ChunkArgs a) {
   using C = Cfg<T, D>;
-  const int lane = threadIdx.x & 63;
   const int hk = blockIdx.x % a.Hkv;
-  const Piece pc = find_piece<C::TR, true>(a, blockIdx.x / a.Hkv, lane);
-  if (!pc.found) return;
+  Piece pc;
+  if (!find_piece<C::TR, C::FEW, true>(a, blockIdx.x / a.Hkv, threadIdx.x & 63, pc)) return;
   const int row0 = pc.tile * C::TR, n_rows = min(pc.rows - row0, C::TR);
   if ((static_cast<int64_t>(pc.slot) + pc.pieces - 1) * a.Hkv + hk >= a.slots || n_rows > a.slot_rows) return;
   const int64_t step = static_cast<int64_t>(a.Hkv) * a.slot_rows;
-  for (int x = threadIdx.x; x < n_rows * (D / 4); x += kThreads) {
+  constexpr int kAhead = 4;
+  const int first = blockIdx.y * kMergeRows, last = min(first + kMergeRows, n_rows);
+  for (int x = threadIdx.x + first * (D / 4); x < last * (D / 4); x += kThreads) {
     const int r = x / (D / 4), d = x % (D / 4) * 4;
     const int64_t base = (static_cast<int64_t>(pc.slot) * a.Hkv + hk) * a.slot_rows + r;
-    float mx = kMasked;
-    for (int s = 0; s < pc.pieces; ++s) mx = fmaxf(mx, a.part_ml[(base + s * step) * 2]);
-    float l = 0.f;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < pc.pieces; ++s) {
-      const float f = __builtin_amdgcn_exp2f(a.part_ml[(base + s * step) * 2] - mx);
-      l = __builtin_fmaf(f, a.part_ml[(base + s * step) * 2 + 1], l);
-      const float4_t o = *reinterpret_cast<const float4_t *>(a.part_o + (base + s * step) * D + d);
+    float mx = kMasked, l = 0.f;
+    float4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < pc.pieces; s0 += kAhead) {
+      float m[kAhead], ls[kAhead];
+      float4_t o[kAhead];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = add_weighted(acc[e], f, o[e]);
+      for (int i = 0; i < kAhead; ++i) {
+        const int64_t at = base + min(s0 + i, pc.pieces - 1) * step;
+        m[i] = a.part_ml[at * 2];
+        ls[i] = a.part_ml[at * 2 + 1];
+        o[i] = *reinterpret_cast<const float4_t *>(a.part_o + at * D + d);
+      }
+      float top = mx;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) top = fmaxf(top, m[i]);  // (the last piece again changes no maximum)
+      const float old = __builtin_amdgcn_exp2f(mx - top);
+      mx = top;
+      l *= old;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = add_weighted(0.f, old, acc[e]);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (s0 + i >= pc.pieces) continue;
+        const float f = __builtin_amdgcn_exp2f(m[i] - top);
+        l = __builtin_fmaf(f, ls[i], l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = add_weighted(acc[e], f, o[i][e]);
+      }
     }
     const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
     const int rr = row0 + r, i = rr / a.group;
@@ -758,8 +820,8 @@ struct Sizes {
   int slot_rows, target;
 };
 // Bounds of the cut for any cu_tokens and start within tokens, B, max_q and max_len.  With q units per piece, q >= work / target
-// and pieces = ceil(units / q) > 1 for a cut tile: its pieces are at most 2 units / q, all cut tiles' together at most
-// 2 work / q <= 2 target.
+// and pieces = ceil(units / p) > 1 for a cut tile, p >= q / 2: its pieces are at most 2 units / p <= 4 units / q, all cut
+// tiles' together at most 4 work / q <= 4 target.
 Sizes sizes_for(int tile_rows, int tokens, int B, int Hkv, int group, int max_q, int max_len) {
   Sizes z{};
   const int64_t rows = static_cast<int64_t>(tokens) * group;
@@ -769,7 +831,7 @@ Sizes sizes_for(int tile_rows, int tokens, int B, int Hkv, int group, int max_q,
   z.target = 2 * device_cu_count();
   const int64_t units = (static_cast<int64_t>(max_len) + 127) / 128;
   const int64_t most = (units + kMinPieceUnits - 1) / kMinPieceUnits;  // pieces of one tile
-  const int64_t cut = 2 * static_cast<int64_t>(z.target) / Hkv + 1;    // pieces of cut tiles, per kv head
+  const int64_t cut = 4 * static_cast<int64_t>(z.target) / Hkv + 1;    // pieces of cut tiles, per kv head
   if (most <= 1) {
     z.grid = z.tiles;
   } else {
@@ -792,7 +854,9 @@ int launch(const ChunkArgs &a, const Sizes &z, hipStream_t st) {
   if (rc != AXHIP_OK) return rc;
   hipLaunchKernelGGL((chunk_attn_kernel<T, D>), dim3(static_cast<unsigned>(z.grid * a.Hkv)), dim3(kThreads), C::kLdsBytes, st, a);
   if (z.cut_tiles > 0)
-    hipLaunchKernelGGL((chunk_merge_kernel<T, D>), dim3(static_cast<unsigned>(z.cut_tiles * a.Hkv)), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((chunk_merge_kernel<T, D>),
+                       dim3(static_cast<unsigned>(z.cut_tiles * a.Hkv), (z.slot_rows + kMergeRows - 1) / kMergeRows), dim3(kThreads), 0,
+                       st, a);
   return launch_status();
 }
 
