@@ -16,7 +16,9 @@
 namespace axhip {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
+constexpr int kAhead = 4;        // loads of a thread on their way at a time
+constexpr int kMostLds = 96 * 1024;
 
 struct LogitsArgs {
   const void *x;
@@ -84,12 +86,18 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
       const int len = a.hist_len ? min(max(a.hist_len[row], 0), a.max_history) : a.max_history;
       const int prompt = a.prompt_len ? max(a.prompt_len[row], 0) : 0;
       const I *ids = static_cast<const I *>(a.history) + row * a.hist_row;
-#pragma unroll 4
-      for (int t = tid; t < len; t += kThreads) {
-        const int64_t id = static_cast<int64_t>(ids[t * a.hist_token]) - v0;
-        if (id >= 0 && id < n) {
-          W::set(static_cast<int>(id), W::kSeen);
-          if (t >= prompt) W::count(static_cast<int>(id));
+      for (int t0 = tid; t0 < len; t0 += kThreads * kAhead) {
+        int64_t id[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) id[u] = ids[min(t0 + u * kThreads, len - 1) * a.hist_token];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int t = t0 + u * kThreads;
+          const int64_t at = id[u] - v0;
+          if (t < len && at >= 0 && at < n) {
+            if (t >= prompt) W::count(static_cast<int>(at));  // (a count says that the token was seen, too)
+            else W::set(static_cast<int>(at), W::kSeen);
+          }
         }
       }
     }
@@ -107,47 +115,56 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
   S *y = static_cast<S *>(a.out) + row * a.out_stride;
   const CT *words = reinterpret_cast<const CT *>(logits_smem);
   const uint32_t *allowed = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-  // whole wavefronts stay in the loop: the search for a bias is theirs together
-  for (int i0 = 0; i0 < n; i0 += kThreads * V) {
-    const int i = i0 + tid * V;
-    const bool on = i < n;  // (a slice ends on a multiple of V, and so does the vocabulary where V > 1)
-    vec in = {};
-    if (on) in = *reinterpret_cast<const vec *>(x + v0 + i);
-    float val[V];
-    uint32_t word[V];
-    uint32_t any = 0;
+  // Whole wavefronts stay in the loop: the search for a bias is
+  // theirs together.
+  for (int i0 = 0; i0 < n; i0 += kThreads * V * kAhead) {
+    vec in[kAhead];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      val[j] = static_cast<float>(in[j]);
-      word[j] = marked && on ? words[i + j] : 0u;
-      any |= word[j];
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + (u * kThreads + tid) * V;  // (a slice ends on a multiple of V, and so does the vocabulary where V > 1)
+      in[u] = {};
+      if (i < n) in[u] = *reinterpret_cast<const vec *>(x + v0 + i);
     }
-    if (__any(any != 0)) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + (u * kThreads + tid) * V;
+      const bool on = i < n;
+      float val[V];
+      uint32_t word[V];
+      uint32_t any = 0;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const uint32_t c = word[j] & W::kCount;
-        if (word[j] & W::kSeen) val[j] = val[j] > 0.f ? val[j] / r : val[j] * r;
-        if (c) val[j] = (val[j] - f * static_cast<float>(c)) - p;
-        for (uint64_t m = __ballot((word[j] & W::kBias) != 0); m; m &= m - 1) {
-          const int l = __ffsll(static_cast<unsigned long long>(m)) - 1;
-          const float b = bias_of(a.bias_ids + static_cast<int64_t>(row) * a.bias_count,
-                                  a.bias + static_cast<int64_t>(row) * a.bias_count, a.bias_count,
-                                  v0 + __builtin_amdgcn_readlane(i, l) + j, lane);
-          if (lane == l) val[j] += b;
+        val[j] = static_cast<float>(in[u][j]);
+        word[j] = marked && on ? words[i + j] : 0u;
+        any |= word[j];
+      }
+      if (__any(any != 0)) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const uint32_t c = word[j] & W::kCount;
+          if (word[j] & (W::kSeen | W::kCount)) val[j] = val[j] > 0.f ? val[j] / r : val[j] * r;
+          if (c) val[j] = (val[j] - f * static_cast<float>(c)) - p;
+          for (uint64_t m = __ballot((word[j] & W::kBias) != 0); m; m &= m - 1) {
+            const int l = __ffsll(static_cast<unsigned long long>(m)) - 1;
+            const float b = bias_of(a.bias_ids + static_cast<int64_t>(row) * a.bias_count,
+                                    a.bias + static_cast<int64_t>(row) * a.bias_count, a.bias_count,
+                                    v0 + __builtin_amdgcn_readlane(i, l) + j, lane);
+            if (lane == l) val[j] += b;
+          }
         }
       }
-    }
-    if (on) {
-      if (allowed) {
-        const uint32_t bits = allowed[(v0 + i) >> 5] >> ((v0 + i) & 31);
+      if (on) {
+        if (allowed) {
+          const uint32_t bits = allowed[(v0 + i) >> 5] >> ((v0 + i) & 31);
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (!((bits >> j) & 1u)) val[j] = -__builtin_inff();
+          for (int j = 0; j < V; ++j)
+            if (!((bits >> j) & 1u)) val[j] = -__builtin_inff();
+        }
+        vec o;
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = static_cast<S>(val[j]);
+        *reinterpret_cast<vec *>(y + v0 + i) = o;
       }
-      vec o;
-#pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = static_cast<S>(val[j]);
-      *reinterpret_cast<vec *>(y + v0 + i) = o;
     }
   }
 }
@@ -157,14 +174,19 @@ int launch(LogitsArgs a, int rows, hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool wide = a.vocab % V == 0 && a.x_stride % V == 0 && a.out_stride % V == 0 &&
                     ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0;
-  // slices: about two workgroups per CU over all rows; at least 2048 tokens each, at most what 64 KB of words hold
-  const int most = 65536 / static_cast<int>(sizeof(CT)), least = 2048;
-  const int64_t want = (2 * device_cu_count() + rows - 1) / rows;
+  // Slices: about one workgroup per CU over all rows, at least 2048 tokens each, at most what 96 KB of words hold.  (64 rows,
+  // 8192 int64 ids each in a [steps, rows] log: 26 us; two workgroups per CU 29 us, since every slice walks the history.)
+  const int most = kMostLds / static_cast<int>(sizeof(CT)), least = 2048;
+  const int64_t want = (device_cu_count() + rows - 1) / rows;
   int64_t slice = (a.vocab + want - 1) / want;
   slice = slice < least ? least : (slice > most ? most : slice);
   a.slice = static_cast<int>((slice + 63) / 64 * 64);
   const dim3 grid(static_cast<unsigned>((a.vocab + a.slice - 1) / a.slice), static_cast<unsigned>(rows));
   const unsigned lds = static_cast<unsigned>(a.slice) * sizeof(CT);
+  static std::atomic<uint64_t> raised[2];
+  const void *kernel = wide ? reinterpret_cast<const void *>(&logits_kernel<T, I, CT, V>) : reinterpret_cast<const void *>(&logits_kernel<T, I, CT, 1>);
+  const int rc = raise_dynamic_lds(kernel, kMostLds, raised[wide]);
+  if (rc != AXHIP_OK) return rc;
   if (wide) hipLaunchKernelGGL((logits_kernel<T, I, CT, V>), grid, dim3(kThreads), lds, st, a);
   else hipLaunchKernelGGL((logits_kernel<T, I, CT, 1>), grid, dim3(kThreads), lds, st, a);
   return launch_status();
