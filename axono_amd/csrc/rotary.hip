@@ -55,13 +55,14 @@ __device__ __forceinline__ void load_v(const T *p, float (&f)[V]) {
 #pragma unroll
   for (int j = 0; j < V; ++j) f[j] = static_cast<float>(x[j]);
 }
-template <typename T, int V>
+template <bool STREAM, typename T, int V>
 __device__ __forceinline__ void store_v(T *p, const float (&f)[V]) {
   typedef Elem<T> vec __attribute__((ext_vector_type(V)));
   vec x;
 #pragma unroll
   for (int j = 0; j < V; ++j) x[j] = static_cast<Elem<T>>(f[j]);
-  *reinterpret_cast<vec *>(p) = x;
+  if constexpr (STREAM) __builtin_nontemporal_store(x, reinterpret_cast<vec *>(p));
+  else *reinterpret_cast<vec *>(p) = x;
 }
 
 // Sum over the 1 << shift lanes of a head.
@@ -92,7 +93,8 @@ __device__ __forceinline__ int sequence_of(const int32_t *cu, int B, int64_t t, 
 }
 
 // V: elements per load; REP: units of 2 V elements a lane takes of a head (more than one only where V is 1 or 2).
-template <typename TI, typename TO, int V, int REP, bool PAGED>
+// STREAM: the results are stored past the caches.
+template <typename TI, typename TO, int V, int REP, bool PAGED, bool STREAM = false>
 __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
   __shared__ float s_cos[kWaves][kMaxPairs], s_sin[kWaves][kMaxPairs];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -113,8 +115,69 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
     }
   }
 
+  // this lane's elements of a head: V from e0[r] on and V from e1[r] on
+  const int units = a.dim / (2 * V), turned = a.rotary_dim / (2 * V), pairs = a.rotary_dim / 2;
+  const int sub = lane & ((1 << a.lanes_shift) - 1);
+  int e0[REP], e1[REP];
+  bool rot[REP], rot1[REP];
+#pragma unroll
+  for (int r = 0; r < REP; ++r) {
+    const int u = sub + 64 * r;
+    if (a.interleaved) {  // chunks u and u + units of the head, V / 2 pairs in each
+      e0[r] = u * V;
+      e1[r] = (u + units) * V;
+      rot[r] = u < units && e0[r] < a.rotary_dim;
+      rot1[r] = u < units && e1[r] < a.rotary_dim;
+    } else {
+      rot[r] = rot1[r] = u < turned;
+      // behind the rotated part the remaining chunks are paired the same way, for the sake of the loads
+      e0[r] = rot[r] ? u * V : a.rotary_dim + (u - turned) * V;
+      e1[r] = rot[r] ? e0[r] + pairs : e0[r] + (units - turned) * V;
+    }
+  }
+
+  const int step = 64 >> a.lanes_shift;
+  const int all = a.heads[0] + a.heads[1] + a.heads[2];
+  const int h_first = group * a.heads_per_group, h_end = min(h_first + a.heads_per_group, all);
+  auto which_of = [&](int h) { return h < a.heads[0] ? 0 : (h < a.heads[0] + a.heads[1] ? 1 : 2); };
+  auto head_in = [&](int h, int which) { return h - (which == 0 ? 0 : (which == 1 ? a.heads[0] : a.heads[0] + a.heads[1])); };
+  // the elements of head h; a head that is not this wavefront's, or has no place to go, reads as zeros
+  auto load = [&](int h, float (&x0)[REP][V], float (&x1)[REP][V]) {
+    const int which = which_of(h), hh = head_in(h, which);
+    const bool live = h < h_end && (!PAGED || which == 0 || cache_row >= 0);
+    const TI *src = static_cast<const TI *>(which == 0 ? a.x[0] : (which == 1 ? a.x[1] : a.x[2])) +
+                    t * (which == 0 ? a.stride[0] : (which == 1 ? a.stride[1] : a.stride[2])) + static_cast<int64_t>(hh) * a.dim;
+#pragma unroll
+    for (int r = 0; r < REP; ++r) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) x0[r][j] = x1[r][j] = 0.f;
+      if (live && sub + 64 * r < units) {
+        load_v<TI, V>(src + e0[r], x0[r]);
+        load_v<TI, V>(src + e1[r], x1[r]);
+      }
+    }
+  };
+  // the first heads, and the weights, are on their way while the angles are made; each next round of heads while one is rotated
+  // (65536 rows into the pages 361 -> 317 us; without norm and pages there is less to wait for, and the registers cost more
+  // wavefronts than the loads ahead bring: 33001 rows 149 us, 159 us with them.)
+  constexpr bool kLoadsAhead = PAGED;
+  float x0[REP][V], x1[REP][V];
+  if constexpr (kLoadsAhead) load(h_first + (lane >> a.lanes_shift), x0, x1);
+  float w0[2][REP][V], w1[2][REP][V];
+  if constexpr (PAGED) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int r = 0; r < REP; ++r)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const bool on = a.norm && a.w[k] && sub + 64 * r < units;
+          w0[k][r][j] = on ? weight_at(a.w[k], a.w_f16, e0[r] + j) : 1.f;
+          w1[k][r][j] = on ? weight_at(a.w[k], a.w_f16, e1[r] + j) : 1.f;
+        }
+  }
+
   // angles: one pair per lane and pass
-  const int pairs = a.rotary_dim / 2;
   for (int i = lane; i < pairs; i += 64) {
     int64_t p = cache_pos;
     if (a.pos) {
@@ -133,68 +196,30 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 
-  // this lane's elements of a head: first[r] .. + V and second[r] .. + V, pair indices first_pair / second_pair
-  const int units = a.dim / (2 * V), turned = a.rotary_dim / (2 * V);
-  const int sub = lane & ((1 << a.lanes_shift) - 1);
-  int e0[REP], e1[REP];
-  float c0[REP][V], n0[REP][V];
-  bool rot[REP], rot1[REP];
+  float c0[REP][V], n0[REP][V];  // interleaved: of the first chunk's pairs, then of the second's
 #pragma unroll
-  for (int r = 0; r < REP; ++r) {
-    const int u = sub + 64 * r;
-    if (a.interleaved) {
-      // chunks u and u + units of the head; V / 2 pairs in each (their cosines: first V / 2 slots, last V / 2)
-      e0[r] = u * V;
-      e1[r] = (u + units) * V;
-      rot[r] = u < units && e0[r] < a.rotary_dim;
-      rot1[r] = u < units && e1[r] < a.rotary_dim;
+  for (int r = 0; r < REP; ++r)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int pair = (j < V / 2 ? e0[r] / 2 + j : e1[r] / 2 + j - V / 2);
-        const bool on = j < V / 2 ? rot[r] : rot1[r];
-        c0[r][j] = on ? s_cos[wave][pair] : 1.f;
-        n0[r][j] = on ? s_sin[wave][pair] : 0.f;
-      }
-    } else {
-      rot[r] = rot1[r] = u < turned;
-      // behind the rotated part the remaining chunks are paired the same way, for the sake of the loads
-      e0[r] = rot[r] ? u * V : a.rotary_dim + (u - turned) * V;
-      e1[r] = rot[r] ? e0[r] + pairs : e0[r] + (units - turned) * V;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        c0[r][j] = rot[r] ? s_cos[wave][u * V + j] : 1.f;
-        n0[r][j] = rot[r] ? s_sin[wave][u * V + j] : 0.f;
-      }
+    for (int j = 0; j < V; ++j) {
+      const bool second = a.interleaved && j >= V / 2;
+      const int pair = a.interleaved ? (second ? e1[r] / 2 + j - V / 2 : e0[r] / 2 + j) : e0[r] + j;
+      const bool on = second ? rot1[r] : rot[r];
+      c0[r][j] = on ? s_cos[wave][pair] : 1.f;
+      n0[r][j] = on ? s_sin[wave][pair] : 0.f;
     }
-  }
 
-  const int step = 64 >> a.lanes_shift;
-  const int all = a.heads[0] + a.heads[1] + a.heads[2];
-  const int h_end = min((group + 1) * a.heads_per_group, all);
   // (every lane stays in the loop: the sums below run over whole rows of lanes)
-  for (int h0 = group * a.heads_per_group; h0 < h_end; h0 += step) {
-    const int h = h0 + (lane >> a.lanes_shift);
-    const int which = h < a.heads[0] ? 0 : (h < a.heads[0] + a.heads[1] ? 1 : 2);
-    const int hh = h - (which == 0 ? 0 : (which == 1 ? a.heads[0] : a.heads[0] + a.heads[1]));
+  for (int h0 = h_first; h0 < h_end; h0 += step) {
+    const int h = h0 + (lane >> a.lanes_shift), which = which_of(h), hh = head_in(h, which);
     const bool live = h < h_end && (!PAGED || which == 0 || cache_row >= 0);
-    const TI *src = static_cast<const TI *>(which == 0 ? a.x[0] : (which == 1 ? a.x[1] : a.x[2])) +
-                    t * (which == 0 ? a.stride[0] : (which == 1 ? a.stride[1] : a.stride[2])) + static_cast<int64_t>(hh) * a.dim;
     TO *dst = static_cast<TO *>(which == 0 ? a.out[0] : (which == 1 ? a.out[1] : a.out[2]));
     if (PAGED && which != 0)
       dst += (cache_row + (static_cast<int64_t>(hh) << kPageShift)) * a.dim;
     else
       dst += (t * (which == 0 ? a.heads[0] : a.heads[1]) + hh) * a.dim;
-    float x0[REP][V], x1[REP][V];
-#pragma unroll
-    for (int r = 0; r < REP; ++r) {
-      const bool on = live && sub + 64 * r < units;
-#pragma unroll
-      for (int j = 0; j < V; ++j) x0[r][j] = x1[r][j] = 0.f;
-      if (on) {
-        load_v<TI, V>(src + e0[r], x0[r]);
-        load_v<TI, V>(src + e1[r], x1[r]);
-      }
-    }
+    float y0[REP][V], y1[REP][V];
+    if constexpr (!kLoadsAhead) load(h, x0, x1);
+    else if (h0 + step < h_end) load(h + step, y0, y1);
     if (PAGED && a.norm) {
       float ss = 0.f;
 #pragma unroll
@@ -202,22 +227,15 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
 #pragma unroll
         for (int j = 0; j < V; ++j) ss = __builtin_fmaf(x0[r][j], x0[r][j], __builtin_fmaf(x1[r][j], x1[r][j], ss));
       ss = head_sum(ss, a.lanes_shift);
-      const void *w = which == 0 ? a.w[0] : a.w[1];
-      if (which < 2 && live) {
+      if (which < 2) {
         const float inv = 1.0f / sqrtf(ss / static_cast<float>(a.dim) + a.eps);
 #pragma unroll
-        for (int r = 0; r < REP; ++r) {
-          if (sub + 64 * r >= units) continue;
+        for (int r = 0; r < REP; ++r)
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            x0[r][j] *= inv;
-            x1[r][j] *= inv;
-            if (w) {
-              x0[r][j] *= weight_at(w, a.w_f16, e0[r] + j);
-              x1[r][j] *= weight_at(w, a.w_f16, e1[r] + j);
-            }
+            x0[r][j] = x0[r][j] * inv * (which == 0 ? w0[0][r][j] : w0[1][r][j]);
+            x1[r][j] = x1[r][j] * inv * (which == 0 ? w1[0][r][j] : w1[1][r][j]);
           }
-        }
       }
     }
 #pragma unroll
@@ -248,8 +266,17 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
           }
         }
       }
-      store_v<TO, V>(dst + e0[r], x0[r]);
-      store_v<TO, V>(dst + e1[r], x1[r]);
+      store_v<STREAM>(dst + e0[r], x0[r]);
+      store_v<STREAM>(dst + e1[r], x1[r]);
+    }
+    if constexpr (kLoadsAhead) {
+#pragma unroll
+      for (int r = 0; r < REP; ++r)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          x0[r][j] = y0[r][j];
+          x1[r][j] = y1[r][j];
+        }
     }
   }
 }
@@ -289,16 +316,20 @@ int launch(RotaryArgs a, hipStream_t st) {
   const int64_t grid = (a.rows * a.groups + kWaves - 1) / kWaves;
   if (grid > INT32_MAX) return AXHIP_INVALID_ARGUMENT;
   const dim3 g(static_cast<unsigned>(grid)), b(kBlock);
-  if constexpr (sizeof(TI) == 2) {
-    if (v == 8) {
-      hipLaunchKernelGGL((rotary_kernel<TI, TO, 8, 1, PAGED>), g, b, 0, st, a);
-      return launch_status();
-    }
-  }
-  switch (v) {
-    case 4: hipLaunchKernelGGL((rotary_kernel<TI, TO, 4, 1, PAGED>), g, b, 0, st, a); break;
-    case 2: hipLaunchKernelGGL((rotary_kernel<TI, TO, 2, 2, PAGED>), g, b, 0, st, a); break;
-    default: hipLaunchKernelGGL((rotary_kernel<TI, TO, 1, 4, PAGED>), g, b, 0, st, a); break;
+  // Results that would push the input of the next operators out of the 256 MB memory-side cache are stored past it (33001 rows
+  // in fp32 150 -> 135 us, 65536 rows into the pages 317 -> 286 us); smaller ones are about to be read again.
+  constexpr int kWide = 16 / sizeof(TI);
+  if (v == kWide) {
+    if (a.rows * all * a.dim * static_cast<int64_t>(sizeof(TO)) >= (int64_t(64) << 20))
+      hipLaunchKernelGGL((rotary_kernel<TI, TO, kWide, 1, PAGED, true>), g, b, 0, st, a);
+    else
+      hipLaunchKernelGGL((rotary_kernel<TI, TO, kWide, 1, PAGED>), g, b, 0, st, a);
+  } else if (v == 4) {
+    if constexpr (kWide > 4) hipLaunchKernelGGL((rotary_kernel<TI, TO, 4, 1, PAGED>), g, b, 0, st, a);
+  } else if (v == 2) {
+    hipLaunchKernelGGL((rotary_kernel<TI, TO, 2, 2, PAGED>), g, b, 0, st, a);
+  } else {
+    hipLaunchKernelGGL((rotary_kernel<TI, TO, 1, 4, PAGED>), g, b, 0, st, a);
   }
   return launch_status();
 }
