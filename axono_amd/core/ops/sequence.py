@@ -4,7 +4,7 @@ axono/python/axono/core/ops/sequence.py); each one hands its arguments to the fu
 from ... import libaxono as _table
 
 __all__ = ["rope", "rope_with_cos_sin", "rope_thd", "mrope_cos_sin", "scaled_dot_product_attention", "embedding",
-           "concat", "slice_", "argmax"]
+           "concat", "slice_", "argmax", "rotary_qk", "rotary_inv_freq", "logits_process"]
 
 
 def rope(x, pos_ids, theta: float = 10000.0):
@@ -28,6 +28,21 @@ def rope_thd(x, pos, inv_freq, mrope_section):
 def mrope_cos_sin(pos, inv_freq, h_sec: int, w_sec: int):
     """The (cos, sin) tables that rope_with_cos_sin needs to do what rope_thd does."""
     return _table.mrope_cos_sin(pos, inv_freq, h_sec, w_sec)
+
+
+def rotary_inv_freq(rotary_dim, theta: float = 10000.0, kind: str = "plain", **scaling):
+    """(table, scale) for rotary_qk: frequencies as they are or scaled for long contexts ("linear", "ntk", "yarn")."""
+    return _table.rotary_inv_freq(rotary_dim, theta, kind, **scaling)
+
+
+def rotary_qk(q, k, pos_ids, inv_freq, scale: float = 1.0, interleaved: bool = False):
+    """q and k (rows, heads, d) rotated by a frequency table: both pair layouts, part of the head."""
+    return _table.rotary_qk(q, k, pos_ids, inv_freq, scale, interleaved)
+
+
+def logits_process(logits, **what):
+    """Penalties for repeated tokens, biases and masks on logits (rows, vocab)."""
+    return _table.logits_process(logits, **what)
 
 
 def scaled_dot_product_attention(q, k, v, is_causal: bool = False):

@@ -142,8 +142,9 @@ def _dev(arr, device):
 
 class Qwen3VLTextDecoder(nn.Module):
     """paged=True keeps the KV cache in pages of 128 keys (nn.PagedKVCache, `n_pages` per layer pool; default:
-    enough for every sequence to reach max_len) instead of one [B, n_kv, max_len, d_head] block per layer; the
-    prefill of a sequence then runs over one dense scratch block and is copied into the sequence's pages."""
+    enough for every sequence to reach max_len) instead of one [B, n_kv, max_len, d_head] block per layer; prefill()
+    of a sequence then runs over one dense scratch block and is copied into the sequence's pages, prefill_chunk() writes and
+    reads the pages themselves."""
 
     def __init__(self, cfg: TextConfig, weights: dict, batch: int, max_len: int, device: str = "hip", paged: bool = False,
                  n_pages: int | None = None, fused_tail: bool | None = None, plan_reuse: bool = True,
@@ -196,6 +197,7 @@ class Qwen3VLTextDecoder(nn.Module):
         if self._fused_tail:
             nbytes = self._lib.axhip_decode_layer_tail_workspace_bytes(cfg.hidden_size, cfg.intermediate_size)
             self._tail_ws = Tensor(DataType.INT8, [nbytes], device)
+        self._sampling = None   # what a step does to its logits before argmax (start_decode)
 
     # ---- pieces ----------------------------------------------------------------------------
     def _w(self, name):
@@ -292,6 +294,8 @@ class Qwen3VLTextDecoder(nn.Module):
         if trace is not None:
             trace.append(h)
         logits = self._linear(xn, "embed_tokens.weight")  # tied lm_head
+        if self._sampling is not None:
+            logits = L.logits_process(logits, **self._sampling)
         return logits, L.argmax(logits)
 
     # ---- prefill -----------------------------------------------------------------------------
@@ -375,15 +379,55 @@ class Qwen3VLTextDecoder(nn.Module):
         logits = self._linear(last_h, "embed_tokens.weight")
         return logits, L.argmax(logits)
 
+    def prefill_chunk(self, new_ids, positions: np.ndarray | None = None):
+        """New tokens of any of the sequences, straight into their pages (paged=True): new_ids[b] are sequence b's (int64, any
+        number of them, none for a sequence that waits), appended at its current length.  So a prompt can be prefilled in
+        chunks, beside sequences that decode, and a conversation continues without a second prefill.  positions: INT64
+        [3, tokens] of the rows in a line (default T = H = W = key position).  Returns (logits FLOAT32 of every sequence's last new
+        token [sequences with tokens, V], their argmax), or (None, None) when no sequence has tokens."""
+        if not self._paged:
+            raise ValueError("prefill_chunk() needs the paged cache (paged=True)")
+        cfg, cache, dev = self._cfg, self._cache, self._device
+        new_ids = [np.ascontiguousarray(x, dtype=np.int64).reshape(-1) for x in new_ids]
+        if len(new_ids) != self._batch:
+            raise ValueError(f"prefill_chunk(): tokens of {self._batch} sequences expected, got {len(new_ids)}")
+        n = np.array([len(x) for x in new_ids], np.int64)
+        T, max_q = int(n.sum()), int(n.max())
+        if T == 0:
+            return None, None
+        cache.reserve(n)
+        cu = _dev(np.concatenate([[0], np.cumsum(n)]).astype(np.int32), dev)
+        pos = _dev(np.ascontiguousarray(positions, dtype=np.int64), dev) if positions is not None else None
+        nqd = cfg.num_attention_heads * cfg.head_dim
+        h = L.embedding(_dev(np.concatenate(new_ids), dev), self._w("embed_tokens.weight")).cast_to(DataType.FLOAT32)
+        xn = L.rms_norm(h, self._w("layers.0.input_layernorm.weight"), cfg.rms_norm_eps, DataType.FLOAT16)
+        for i in range(cfg.num_hidden_layers):
+            p = f"layers.{i}."
+            q = cache.append_chunk(i, self._linear(xn, p + "self_attn.qkv_proj.weight"), cfg.num_attention_heads, self._inv_freq, cu,
+                                   pos=pos, mrope_section=cfg.mrope_section, q_weight=self._w(p + "self_attn.q_norm.weight"),
+                                   k_weight=self._w(p + "self_attn.k_norm.weight"), eps=cfg.rms_norm_eps)
+            attn = cache.attend_chunk(i, q, cu, max_q).reshape([T, nqd])
+            h, xn2 = L.add_rms_norm(self._linear(attn, p + "self_attn.o_proj.weight"), h,
+                                    self._w(p + "post_attention_layernorm.weight"), cfg.rms_norm_eps, DataType.FLOAT16)
+            nxt = f"layers.{i + 1}.input_layernorm.weight" if i + 1 < cfg.num_hidden_layers else "norm.weight"
+            h, xn = L.add_rms_norm(self._mlp(xn2, p), h, self._w(nxt), cfg.rms_norm_eps, DataType.FLOAT16)
+        cache.advance_each(n)
+        last = np.cumsum(n)[n > 0] - 1   # rows of the last new tokens
+        logits = self._linear(L.embedding(_dev(last, dev), xn), "embed_tokens.weight")
+        return logits, L.argmax(logits)
+
     # ---- captured decode loop ------------------------------------------------------------------
     def start_decode(self, first_ids: np.ndarray, first_pos: np.ndarray, max_new_tokens: int,
-                     trace: list | None = None):
+                     trace: list | None = None, sampling: dict | None = None):
         """Sets the static step inputs (ids [B], positions [3,B]) and captures the step.  The
         attention split plan is sized for the lengths the loop will reach.  `trace`, if given, holds
         after every run of the step (eager, or a replay of the captured one) the residual stream entering
         each layer and the one leaving the last, as decode_forward documents; inside a captured step these
-        are the graph's own buffers, refreshed by each replay."""
+        are the graph's own buffers, refreshed by each replay.  `sampling`, if given, holds what every step does to its
+        logits before argmax: keywords of libaxono.logits_process (repetition, presence, frequency, bias_ids, bias, allowed;
+        device tensors, read again by every replay), with the tokens of the loop so far as the history."""
         B = self._batch
+        self._sampling = None
         self._ids.copy_from_numpy(np.ascontiguousarray(first_ids, dtype=np.int64).reshape(B))
         self._pos.copy_from_numpy(np.ascontiguousarray(first_pos, dtype=np.int64).reshape(3, B))
         bound = min(self._cache.max_len, len(self._cache) + max_new_tokens + 1)
@@ -397,6 +441,9 @@ class Qwen3VLTextDecoder(nn.Module):
         # the tokens of every step are gathered on the device, at the row a device-side counter names
         self._log = Tensor(DataType.INT64, [max(max_new_tokens, 1), B], self._device)
         self._counter = Tensor(DataType.INT64, [1], self._device)
+        self._logged = Tensor(DataType.INT32, [B], self._device)   # rows of the log that hold tokens, for the history
+        if sampling is not None:
+            self._sampling = {**sampling, "history": self._log, "history_len": self._logged, "by_step": True}
 
         def step():
             if trace is not None:
@@ -404,6 +451,8 @@ class Qwen3VLTextDecoder(nn.Module):
             logits, nxt = self.decode_forward(self._ids, self._pos, bound, trace=trace)
             # the device-side state of the next step, and the token log: one launch
             L.decode_advance(nxt, self._ids, self._pos, self._cache.seq_lens, self._log, self._counter)
+            if sampling is not None:
+                L.index_add(self._logged, 1)
             return logits, nxt
 
         self._step_fn = step
@@ -421,6 +470,7 @@ class Qwen3VLTextDecoder(nn.Module):
         self._pos.copy_from_numpy(pos0)
         self._cache.seq_lens.copy_from_numpy(lens0)
         self._counter.copy_from_numpy(np.zeros(1, np.int64))
+        self._logged.fill_zero()
         self._graph = g
         self._graph_out = g.outputs
         return g
@@ -439,6 +489,7 @@ class Qwen3VLTextDecoder(nn.Module):
                                f"{self._decode_bound} keys; {have} cached + {max_new_tokens} new exceed that. "
                                f"Call start_decode() (and capture()) again for the new length")
         self._counter.copy_from_numpy(np.zeros(1, np.int64))
+        self._logged.fill_zero()
         L.synchronize()
         for _ in range(max_new_tokens):
             if use_graph:

@@ -11,6 +11,8 @@ from __future__ import annotations
 
 import ctypes as C
 
+import numpy as np
+
 from . import _lib
 from .core.tensor import Tensor, hip_available
 from .core.types import DataType, Status
@@ -36,6 +38,12 @@ def _need_hip(op: str, *tensors) -> None:
             dev = t._dev_id
         elif t._dev_id != dev:
             raise AxhipError(op, Status.DEVICE_MISMATCH)
+
+
+def _use_device(op: str, like: Tensor) -> None:
+    # creating a result selects its device; a call whose results are given has to do it itself
+    if like.num_elements:
+        check(_lib_().axhip_set_device(like._dev_id), op)
 
 
 def _new(dtype, shape, like: Tensor) -> Tensor:
@@ -562,6 +570,60 @@ def argmax(x: Tensor) -> Tensor:
     return out
 
 
+def logits_process(logits: Tensor, history: Tensor | None = None, history_len: Tensor | None = None,
+                   prompt_len: Tensor | None = None, repetition: Tensor | None = None, presence: Tensor | None = None,
+                   frequency: Tensor | None = None, bias_ids: Tensor | None = None, bias: Tensor | None = None,
+                   allowed: Tensor | None = None, by_step: bool = False, out: Tensor | None = None) -> Tensor:
+    """Penalties, biases and a grammar's mask on logits (rows, vocab), before argmax or sampling.  In this order: a token in
+    the row's history is divided by `repetition` where its logit is positive and multiplied where not; frequency * count +
+    presence is taken off a token with count > 0 occurrences behind the prompt; bias entries (bias_ids INT32, bias FLOAT32, both
+    (rows, n)) are added; tokens whose bit of `allowed` (INT32 (rows, words), bit v % 32 of word v / 32) is 0 become -inf.
+    history: INT32 / INT64 ids (rows, H), or (H, rows) with by_step - the token log of decode_advance; history_len, prompt_len
+    INT32 (rows,); repetition, presence, frequency FLOAT32 (rows,).  out may be logits."""
+    op = "logits_process"
+    _need_hip(op, logits, history, history_len, prompt_len, repetition, presence, frequency, bias_ids, bias, allowed, out)
+    if logits.ndim < 1 or logits.dtype not in _FLOATS:
+        raise AxhipError(op, Status.UNSUPPORTED_TYPE)
+    vocab = logits.shape[-1]
+    rows = logits.num_elements // vocab if vocab else 0
+    H = 0
+    if history is not None:
+        if history.dtype not in (DataType.INT32, DataType.INT64):
+            raise AxhipError(op, Status.UNSUPPORTED_TYPE)
+        if history.ndim != 2 or history.shape[1 if by_step else 0] != rows:
+            raise AxhipError(op, Status.SHAPE_MISMATCH)
+        H = history.shape[0 if by_step else 1]
+    for t, dt in ((history_len, DataType.INT32), (prompt_len, DataType.INT32), (repetition, DataType.FLOAT32),
+                  (presence, DataType.FLOAT32), (frequency, DataType.FLOAT32)):
+        if t is not None and (t.dtype != dt or t.num_elements != rows):
+            raise AxhipError(op, Status.SHAPE_MISMATCH)
+    n_bias = 0
+    if (bias_ids is None) != (bias is None):
+        raise AxhipError(op, Status.INVALID_ARGUMENT)
+    if bias_ids is not None:
+        if bias_ids.dtype != DataType.INT32 or bias.dtype != DataType.FLOAT32:
+            raise AxhipError(op, Status.UNSUPPORTED_TYPE)
+        if bias_ids.ndim != 2 or bias_ids.shape[0] != rows or bias.shape != bias_ids.shape:
+            raise AxhipError(op, Status.SHAPE_MISMATCH)
+        n_bias = bias_ids.shape[1]
+    if allowed is not None and (allowed.dtype != DataType.INT32 or allowed.ndim != 2 or allowed.shape[0] != rows or
+                                allowed.shape[1] * 32 < vocab):
+        raise AxhipError(op, Status.SHAPE_MISMATCH)
+    if out is None:
+        out = _new(logits.dtype, logits.shape, logits)
+    elif out.shape != logits.shape or out.dtype != logits.dtype:
+        raise AxhipError(op, Status.SHAPE_MISMATCH)
+    _use_device(op, logits)
+    ptr = lambda t: t.data_ptr if t is not None else None
+    by_row, by_token = (1, rows) if by_step else (H, 1)
+    check(_lib_().axhip_logits_process(
+        logits.data_ptr, vocab, int(logits.dtype), ptr(history), int(history.dtype) if history is not None else int(DataType.INT32),
+        by_row, by_token, H, ptr(history_len), ptr(prompt_len), ptr(repetition), ptr(presence), ptr(frequency), ptr(bias_ids),
+        ptr(bias), n_bias, ptr(allowed), allowed.shape[1] if allowed is not None else 0, out.data_ptr, vocab, rows, vocab,
+        current_stream()), op)
+    return out
+
+
 # ---- glue of the captured decode step -------------------------------------------------------------
 def index_add(x: Tensor, delta: int) -> Tensor:
     """x += delta in place (INT32 / INT64), on the device."""
@@ -874,6 +936,147 @@ def kv_dense_to_paged(k_dense: Tensor, v_dense: Tensor, k_pool: Tensor, v_pool: 
     check(_lib_().axhip_kv_dense_to_paged(k_dense.data_ptr, v_dense.data_ptr, k_pool.data_ptr, v_pool.data_ptr, tbl, lens_ptr,
                                           k_pool.num_bytes // max(k_pool.num_elements, 1), B, hkv, rows, d, max_pages, n_pages,
                                           current_stream()), op)
+
+
+# ---- new tokens of a ragged batch over a paged cache ---------------------------------------------
+# `tokens` rows in a line: those of sequence b are cu_tokens[b] .. cu_tokens[b + 1] (INT32 [B + 1]), the first of them sits at key
+# position start[b] (INT32 [B]); both on the device, where the kernels read them.
+ROTARY_KINDS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+
+def rotary_inv_freq(rotary_dim: int, theta: float = 10000.0, kind: str = "plain", factor: float = 1.0, trained_len: int = 0,
+                    fast_turns: float = 32.0, slow_turns: float = 1.0, device: str = "hip"):
+    """The frequency table of rotary_qk / rotary_append_paged, FLOAT32 (rotary_dim / 2,) on `device`, and the factor on
+    cosine and sine that belongs to it: theta^(-2i / rotary_dim) as it is ("plain"), divided by `factor` ("linear"), with
+    theta raised ("ntk"), or with the slow frequencies divided and the fast ones kept ("yarn": between slow_turns and
+    fast_turns turns over trained_len positions)."""
+    op = "rotary_inv_freq"
+    if kind not in ROTARY_KINDS:
+        raise ValueError(f"rotary_inv_freq: kind must be one of {sorted(ROTARY_KINDS)}, got {kind!r}")
+    if int(rotary_dim) <= 0:
+        raise AxhipError(op, Status.INVALID_ARGUMENT)
+    table, scale = np.zeros(int(rotary_dim) // 2, np.float32), C.c_float(1.0)
+    check(_lib_().axhip_rotary_inv_freq(ROTARY_KINDS[kind], float(theta), int(rotary_dim), float(factor), int(trained_len),
+                                        float(fast_turns), float(slow_turns), table.ctypes.data, C.byref(scale)), op)
+    return Tensor.from_numpy_ref(table).to(device), float(scale.value)
+
+
+def _rotary_table(op, inv_freq, d):
+    if inv_freq.dtype != DataType.FLOAT32 or inv_freq.ndim != 1 or not 0 < 2 * inv_freq.num_elements <= d:
+        raise AxhipError(op, Status.SHAPE_MISMATCH)
+    return 2 * inv_freq.num_elements
+
+
+def rotary_qk(q: Tensor, k: Tensor | None, pos_ids: Tensor, inv_freq: Tensor, scale: float = 1.0, interleaved: bool = False):
+    """q (rows, Hq, d) and k (rows, Hk, d) or None, rotated at INT64 positions (rows,) by a table of frequencies
+    (rotary_inv_freq): the first 2 * len(inv_freq) elements of every head, as pairs (i, i + half) or, interleaved,
+    (2i, 2i + 1); the rest is copied.  Angles in 64 bits.  Returns (q_out, k_out)."""
+    op = "rotary_qk"
+    _need_hip(op, q, k, pos_ids, inv_freq)
+    for x in (q, k):
+        if x is not None and (x.ndim != 3 or x.dtype not in _FLOATS):
+            raise AxhipError(op, Status.UNSUPPORTED_TYPE)
+    rows, hq, d = q.shape
+    if k is not None and (k.shape[0] != rows or k.shape[2] != d or k.dtype != q.dtype):
+        raise AxhipError(op, Status.SHAPE_MISMATCH)
+    if pos_ids.dtype != DataType.INT64:
+        raise AxhipError(op, Status.UNSUPPORTED_TYPE)
+    if pos_ids.num_elements != rows:
+        raise AxhipError(op, Status.SHAPE_MISMATCH)
+    rd, hk = _rotary_table(op, inv_freq, d), k.shape[1] if k is not None else 0
+    qo, ko = _new(q.dtype, q.shape, q), _new(k.dtype, k.shape, k) if k is not None else None
+    check(_lib_().axhip_rotary_qk(q.data_ptr, hq * d, k.data_ptr if k is not None else None, hk * d, pos_ids.data_ptr,
+                                  inv_freq.data_ptr, float(scale), 1 if interleaved else 0, rd, qo.data_ptr,
+                                  ko.data_ptr if ko is not None else None, int(q.dtype), rows, hq, hk, d, current_stream()), op)
+    return qo, ko
+
+
+def _ragged_check(op, cu_tokens, start, page_table, k_pool, v_pool):
+    if k_pool.ndim != 4 or k_pool.dtype not in _FLOATS or v_pool.dtype != k_pool.dtype:
+        raise AxhipError(op, Status.UNSUPPORTED_TYPE)
+    if cu_tokens.dtype != DataType.INT32 or start.dtype != DataType.INT32 or page_table.dtype != DataType.INT32:
+        raise AxhipError(op, Status.UNSUPPORTED_TYPE)
+    B = start.num_elements
+    if v_pool.shape != k_pool.shape or k_pool.shape[2] != PAGE_KEYS or cu_tokens.num_elements != B + 1 or page_table.ndim != 2 or \
+            page_table.shape[0] != B:
+        raise AxhipError(op, Status.SHAPE_MISMATCH)
+    return B
+
+
+def rotary_append_paged(qkv: Tensor, n_q_heads: int, inv_freq: Tensor, cu_tokens: Tensor, start: Tensor, k_pool: Tensor,
+                        v_pool: Tensor, page_table: Tensor, pos: Tensor | None = None, scale: float = 1.0,
+                        interleaved: bool = False, mrope_section=None, q_weight: Tensor | None = None,
+                        k_weight: Tensor | None = None, eps: float | None = None) -> Tensor:
+    """qkv (tokens, (Hq + 2 Hkv) * D), the fused projection of the new tokens of a ragged batch: the q and k heads are
+    normalised over D when eps is given (weights optional), rotated as in rotary_qk, k and v written to their rows of the paged
+    cache (pools (n_pages, Hkv, 128, D), page_table INT32 (B, max_pages)).  Returns q (tokens, Hq, D) in the pools' type.
+    pos: INT64 (tokens,), or (3, tokens) with mrope_section = (t, h, w) sizes, or None: the key positions."""
+    op = "rotary_append_paged"
+    _need_hip(op, qkv, inv_freq, cu_tokens, start, k_pool, v_pool, page_table, pos, q_weight, k_weight)
+    if qkv.dtype not in _FLOATS or qkv.ndim < 1:
+        raise AxhipError(op, Status.UNSUPPORTED_TYPE)
+    B = _ragged_check(op, cu_tokens, start, page_table, k_pool, v_pool)
+    n_pages, hkv, _, d = k_pool.shape
+    hq = int(n_q_heads)
+    width = (hq + 2 * hkv) * d
+    tokens = qkv.shape[0]
+    if hq <= 0 or qkv.num_elements != tokens * width:
+        raise AxhipError(op, Status.SHAPE_MISMATCH)
+    axes = 1
+    if pos is not None:
+        axes = 3 if pos.ndim == 2 else 1
+        if pos.dtype != DataType.INT64:
+            raise AxhipError(op, Status.UNSUPPORTED_TYPE)
+        if pos.shape != ([3, tokens] if axes == 3 else [tokens]):
+            raise AxhipError(op, Status.SHAPE_MISMATCH)
+    for w in (q_weight, k_weight):
+        if w is not None and (eps is None or w.num_elements != d or w.dtype not in _FLOATS):
+            raise AxhipError(op, Status.SHAPE_MISMATCH)
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise AxhipError(op, Status.UNSUPPORTED_TYPE)
+    rd = _rotary_table(op, inv_freq, d)
+    _, h_sec, w_sec = (list(mrope_section or []) + [0, 0, 0])[:3]
+    q_out = _new(k_pool.dtype, [tokens, hq, d], qkv)
+    base, esz = qkv.data_ptr, qkv.num_bytes // max(qkv.num_elements, 1)
+    w = q_weight if q_weight is not None else k_weight
+    ptr = lambda t: t.data_ptr if t is not None else None
+    check(_lib_().axhip_rotary_append_paged(
+        base, width, base + hq * d * esz, width, base + (hq + hkv) * d * esz, width, int(qkv.dtype), ptr(q_weight), ptr(k_weight),
+        int(w.dtype) if w is not None else int(DataType.FLOAT32), float(eps or 0.0), 1 if eps is not None else 0, ptr(pos), axes,
+        inv_freq.data_ptr, float(scale), 1 if interleaved else 0, rd, int(h_sec), int(w_sec), cu_tokens.data_ptr, start.data_ptr,
+        page_table.data_ptr, q_out.data_ptr, k_pool.data_ptr, v_pool.data_ptr, int(k_pool.dtype), tokens, B, hq, hkv, d,
+        page_table.shape[1], n_pages, current_stream()), op)
+    return q_out
+
+
+def chunk_attention_paged(q: Tensor, k_pool: Tensor, v_pool: Tensor, page_table: Tensor, cu_tokens: Tensor, start: Tensor,
+                          max_q: int, max_len: int, out: Tensor | None = None, workspace: Tensor | None = None) -> Tensor:
+    """Causal attention of the new tokens of a ragged batch, q (tokens, Hq, D), over the paged cache that already holds their
+    keys and values (rotary_append_paged): the i-th new token of sequence b sees keys 0 .. start[b] + i.  From one token a
+    sequence to chunks of a prompt, mixed in one call.  max_q bounds the new tokens of a sequence, max_len its keys with
+    them.  A workspace that is passed in serves launches that do not overlap in time."""
+    op = "chunk_attention_paged"
+    _need_hip(op, q, k_pool, v_pool, page_table, cu_tokens, start, out, workspace)
+    if q.ndim != 3 or q.dtype not in _FLOATS or k_pool.dtype != q.dtype:
+        raise AxhipError(op, Status.UNSUPPORTED_TYPE)
+    B = _ragged_check(op, cu_tokens, start, page_table, k_pool, v_pool)
+    tokens, hq, d = q.shape
+    n_pages, hkv, _, dk = k_pool.shape
+    if dk != d or hkv == 0 or hq % hkv != 0:
+        raise AxhipError(op, Status.SHAPE_MISMATCH)
+    if out is None:
+        out = _new(q.dtype, [tokens, hq, d], q)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise AxhipError(op, Status.SHAPE_MISMATCH)
+    _use_device(op, q)
+    lib = _lib_()
+    sizes = (int(q.dtype), tokens, B, hq, hkv, d, int(max_q), int(max_len))
+    need = lib.axhip_chunk_attention_paged_workspace_bytes(*sizes)
+    ws = workspace if workspace is not None else _workspace(need, q)
+    check(lib.axhip_chunk_attention_paged(q.data_ptr, k_pool.data_ptr, v_pool.data_ptr, page_table.data_ptr, cu_tokens.data_ptr,
+                                          start.data_ptr, out.data_ptr, ws.data_ptr, ws.num_bytes, *sizes, page_table.shape[1],
+                                          n_pages, current_stream()), op)
+    return out
 
 
 # ---- graph capture -------------------------------------------------------------------------------

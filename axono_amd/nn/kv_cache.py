@@ -302,6 +302,26 @@ class PagedKVCache(KVCache):
         return _l.gqa_decode_attention_paged(q, self._k[layer_idx], self._v[layer_idx], self.page_table, lens,
                                              max(min(bound, self.max_len), 1))
 
+    # ---- ragged batches of new tokens ------------------------------------------------------------
+    def append_chunk(self, layer_idx: int, qkv, n_q_heads: int, inv_freq, cu_tokens, **rotary):
+        """New tokens of a ragged batch (rows cu_tokens[b] .. cu_tokens[b + 1] of the fused projection qkv are sequence b's): norm
+        and rotation of q and k, k and v written behind every sequence's current length; returns q.  Pages for them
+        must be there (`reserve`).  Keywords as in libaxono.rotary_append_paged."""
+        return _l.rotary_append_paged(qkv, n_q_heads, inv_freq, cu_tokens, self.seq_lens, self._k[layer_idx], self._v[layer_idx],
+                                      self.page_table, **rotary)
+
+    def attend_chunk(self, layer_idx: int, q, cu_tokens, max_q: int, max_len: int | None = None, workspace=None):
+        """Causal attention of the tokens that `append_chunk` has written (and `advance_rows` / `advance` not yet counted): max_q
+        bounds the new tokens of a sequence.  Runs on the device; a captured call passes the longest max_len it will see."""
+        bound = int(max_len) if max_len is not None else int(self._lens.max()) + int(max_q)
+        return _l.chunk_attention_paged(q, self._k[layer_idx], self._v[layer_idx], self.page_table, cu_tokens, self.seq_lens, max_q,
+                                        max(min(bound, self.max_len), 1), workspace=workspace)
+
+    def advance_each(self, new_tokens) -> None:
+        """Sequence b grew by new_tokens[b] (after the last layer of a ragged batch)."""
+        self._lens += np.asarray(new_tokens, np.int64).reshape(self.batch)
+        self.seq_lens.copy_from_numpy(self._lens.astype(np.int32))
+
     def set_lengths(self, lens) -> None:
         """Sets every sequence's length (pages for them must exist: `reserve` / `update_rows` first)."""
         lens = np.ascontiguousarray(lens, dtype=np.int64).reshape(self.batch)

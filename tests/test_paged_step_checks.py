@@ -143,3 +143,24 @@ def test_frequency_table_refusals():
         assert inv_freq(*bad)[0] == INVALID, bad
     assert lib().axhip_rotary_inv_freq(0, 1e4, 63, 1.0, 0, 0.0, 0.0, P, None) == INVALID
     assert lib().axhip_rotary_inv_freq(0, 1e4, 64, 1.0, 0, 0.0, 0.0, None, None) == PTR
+
+
+def test_host_tensors_are_refused():
+    from axono_amd import Status, Tensor, libaxono as L
+    from axono_amd.device import AxhipError
+
+    def host(shape, t=np.float32):
+        return Tensor.from_numpy_ref(np.zeros(shape, t))
+
+    f, i32 = host(32), np.int32
+    pools = (host((2, 1, 128, 64), np.float16),) * 2
+    ragged = (host(2, i32), host(1, i32))
+    for call in (lambda: L.rotary_qk(host((3, 2, 64)), None, host(3, np.int64), f),
+                 lambda: L.rotary_append_paged(host((3, 256)), 2, f, *ragged, *pools, host((1, 2), i32)),
+                 lambda: L.chunk_attention_paged(host((3, 2, 64), np.float16), *pools, host((1, 2), i32), *ragged, 3, 128),
+                 lambda: L.logits_process(host((2, 100)))):
+        with pytest.raises(AxhipError) as e:
+            call()
+        assert e.value.code == Status.DEVICE_MISMATCH
+    table, scale = L.rotary_inv_freq(64, 1e4, "linear", factor=2.0, device="cpu")
+    assert scale == 1.0 and table.shape == [32] and abs(float(table.to_numpy()[0]) - 0.5) < 1e-7
