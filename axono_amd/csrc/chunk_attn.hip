@@ -463,8 +463,11 @@ struct Wave {
     }
   }
   // The units that this thread has fetched are in LDS, and clean.  (The barrier behind this call makes them everybody's.)
+  // NEXT: another stage's loads have been issued since, and stay under way.
+  template <bool NEXT = false>
   __device__ __forceinline__ void stage_arrived(int key0, int buf) const {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (NEXT) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C::VEC) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (key0 + KS > mixed_from) {  // uniform
       bool bad = false;
 #pragma unroll 1
@@ -478,14 +481,20 @@ struct Wave {
   __device__ __forceinline__ void shared_stages(bool few) {
     const int n_stages = k_end > k0 ? (k_end - k0 + KS - 1) / KS : 0;
     const bool idle = wrow >= n_rows;  // a wavefront without rows only loads
-    if (n_stages > 0) load_stage(page_of(k0), k0, 0);
-    load_q();
-    __syncthreads();  // the flag is cleared
     if (n_stages == 0) return;
-    stage_arrived(k0, 0);
-    lds_barrier();
-    if (n_stages > 1) load_stage(page_of(k0 + KS), k0 + KS, 1);
+    const int page0 = page_of(k0), page1 = page_of(k0 + KS);
     int s = 0, page = page_of(k0 + 2 * KS);
+    load_q();
+    asm volatile("" ::: "memory");  // the queries' loads are issued before the stages'
+    load_stage(page0, k0, 0);
+    lds_barrier();  // the flag is cleared
+    if (n_stages > 1) {
+      load_stage(page1, k0 + KS, 1);
+      stage_arrived<true>(k0, 0);
+    } else {
+      stage_arrived(k0, 0);
+    }
+    lds_barrier();
     // Stages that every row of the tile sees whole run as a software pipeline: while one block's scores and values are
     // multiplied, the next operands come from LDS, so a wavefront never waits for an LDS read that it has just made.  The
     // barrier that ends a stage stands in the middle of its last block, behind that block's last LDS read.
@@ -593,13 +602,15 @@ struct Wave {
   }
   __device__ __forceinline__ void own_blocks() {
     constexpr int kHop = kWavesWg * kBlockKeys;
-    load_q();
-    __syncthreads();  // the flag is cleared
+    lds_barrier();  // the flag is cleared
     int kb = k0 + wave * kBlockKeys;
     if (kb >= k_end) return;
-    KFrag now[2][QF], next[2][QF];
-    fetch_own(page_of(kb), kb, 0, now);
+    const int page0 = page_of(kb);
     int page = page_of(kb + kHop);
+    load_q();
+    asm volatile("" ::: "memory");  // the queries' loads are issued before the keys'
+    KFrag now[2][QF], next[2][QF];
+    fetch_own(page0, kb, 0, now);
 #pragma unroll 1
     for (int buf = 0;; buf ^= 1) {
       // the block in use has arrived when no more than the next one's loads are under way (loads return in order)
