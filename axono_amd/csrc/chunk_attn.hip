@@ -36,7 +36,6 @@ constexpr int kPageKeys = 128, kPageShift = 7;
 constexpr int kBlockKeys = 32;      // keys of one softmax step
 constexpr float kMasked = -1.0e30f;
 typedef float float8_t __attribute__((ext_vector_type(8)));
-constexpr int kMinPieceUnits = 2;   // a piece has at least 2 units of 128 keys
 
 struct ChunkArgs {
   const void *q, *k, *v;
@@ -51,7 +50,13 @@ struct ChunkArgs {
 
 template <typename T, int D>
 struct Cfg {
-  static constexpr int NT = D == 256 || (sizeof(T) == 4 && D == 128) ? 1 : 2;  // column tiles per wavefront
+  // Column tiles per wavefront, and the fewest units of 128 keys of a piece.  fp32 products take long enough for one
+  // column tile, and with half the rows in a tile and pieces of a single unit small batches spread over more workgroups
+  // (D = 64; before: 2 and 2): 3 ragged prompts of 200 tokens 17 us against 29, 16 decoding sequences at 2000 keys 29
+  // against 39; against that 4 x 1000 tokens at 2000 keys 321 us against 314, 4096 tokens of one prompt 254 against 220.
+  // fp16 is slower with pieces of one unit (512 tokens of one prompt 25 us against 23) and gains nothing from it.
+  static constexpr int NT = D == 256 || sizeof(T) == 4 ? 1 : 2;
+  static constexpr int MIN = sizeof(T) == 4 ? 1 : 2;
   static constexpr int TR = kWavesWg * 16 * NT;                        // rows per tile
   static constexpr int FEW = 16 * NT;                                  // rows up to which wavefronts deal the keys
   static constexpr int KS = (D == 256 || (sizeof(T) == 4 && D == 128)) ? 32 : 64;  // keys per stage
@@ -94,21 +99,21 @@ __device__ __forceinline__ int last_key(const ChunkArgs &a, int start, int r) {
   return static_cast<int>(p < -1 ? -1 : (p > a.max_len - 1 ? a.max_len - 1 : p));
 }
 // Units per piece: the work of a kv head (every tile taken as long as its sequence's last) over the pieces aimed at.
-template <int TR>
+template <typename C>
 __device__ __forceinline__ int units_per_piece(const ChunkArgs &a, const Seq &first, int lane) {
   float work = 0.f;
   for (int j = 0; j < a.B; j += 64) {
-    const Seq s = j == 0 ? first : load_seq<TR>(a, j + lane);
+    const Seq s = j == 0 ? first : load_seq<C::TR>(a, j + lane);
     work += group_sum<64>(static_cast<float>(s.tiles) * static_cast<float>(s.units));
   }
   const float q = ceilf(work * static_cast<float>(a.Hkv) / static_cast<float>(a.target));
-  return __builtin_amdgcn_readfirstlane(max(kMinPieceUnits, static_cast<int>(fminf(q, 1.0e9f))));
+  return __builtin_amdgcn_readfirstlane(max(C::MIN, static_cast<int>(fminf(q, 1.0e9f))));
 }
 // Pieces of every tile of a sequence.  One that has few rows only streams keys, each its own: shorter pieces spread such
 // streams better over the device, while tiles of many rows that start together share their keys in the caches.
 template <typename C>
 __device__ __forceinline__ int pieces_of(const Seq &s, int per) {
-  const int p = C::kOwnBlocks && s.rows <= C::FEW ? max(kMinPieceUnits, (per + 1) / 2) : per;
+  const int p = C::kOwnBlocks && s.rows <= C::FEW ? max(C::MIN, (per + 1) / 2) : per;
   return max(1, (s.units + p - 1) / p);
 }
 
@@ -120,7 +125,7 @@ struct Piece {
 template <typename C, bool MERGE>
 __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int flat, int lane, Piece &p) {
   const Seq first = load_seq<C::TR>(a, lane);
-  const int per = units_per_piece<C::TR>(a, first, lane);
+  const int per = units_per_piece<C>(a, first, lane);
   int done = 0, slots = 0;
   for (int j = 0; j < a.B; j += 64) {
     const Seq s = j == 0 ? first : load_seq<C::TR>(a, j + lane);
@@ -840,18 +845,30 @@ struct Sizes {
   int64_t cut_tiles;  // cut tiles at most, per kv head
   int slot_rows, target;
 };
+struct Tile {
+  int rows, min_units;
+};
+template <typename T>
+Tile tile_for(int D) {
+  if (D == 64) return {Cfg<T, 64>::TR, Cfg<T, 64>::MIN};
+  if (D == 128) return {Cfg<T, 128>::TR, Cfg<T, 128>::MIN};
+  return {Cfg<T, 256>::TR, Cfg<T, 256>::MIN};
+}
+Tile tile_of(int dtype, int D) { return dtype == AXHIP_FLOAT32 ? tile_for<float>(D) : tile_for<__half>(D); }
+
 // Bounds of the cut for any cu_tokens and start within tokens, B, max_q and max_len.  With q units per piece, q >= work / target
 // and pieces = ceil(units / p) > 1 for a cut tile, p >= q / 2: its pieces are at most 2 units / p <= 4 units / q, all cut
 // tiles' together at most 4 work / q <= 4 target.
-Sizes sizes_for(int tile_rows, int tokens, int B, int Hkv, int group, int max_q, int max_len) {
+Sizes sizes_for(Tile tile, int tokens, int B, int Hkv, int group, int max_q, int max_len) {
   Sizes z{};
+  const int tile_rows = tile.rows;
   const int64_t rows = static_cast<int64_t>(tokens) * group;
   z.tiles = rows / tile_rows + B;
   const int64_t per_seq = (static_cast<int64_t>(max_q) * group + tile_rows - 1) / tile_rows;
   if (z.tiles > per_seq * B) z.tiles = per_seq * B;
   z.target = 2 * device_cu_count();
   const int64_t units = (static_cast<int64_t>(max_len) + 127) / 128;
-  const int64_t most = (units + kMinPieceUnits - 1) / kMinPieceUnits;  // pieces of one tile
+  const int64_t most = (units + tile.min_units - 1) / tile.min_units;  // pieces of one tile
   const int64_t cut = 4 * static_cast<int64_t>(z.target) / Hkv + 1;    // pieces of cut tiles, per kv head
   if (most <= 1) {
     z.grid = z.tiles;
@@ -865,8 +882,6 @@ Sizes sizes_for(int tile_rows, int tokens, int B, int Hkv, int group, int max_q,
   }
   return z;
 }
-int tile_rows_of(int dtype, int D) { return D == 256 || (dtype == AXHIP_FLOAT32 && D == 128) ? 64 : 128; }
-
 template <typename T, int D>
 int launch(const ChunkArgs &a, const Sizes &z, hipStream_t st) {
   using C = Cfg<T, D>;
@@ -908,7 +923,7 @@ AXHIP_API size_t axhip_chunk_attention_paged_workspace_bytes(int dtype, int toke
                                                              int max_len) {
   if (check_sizes(dtype, tokens, B, Hq, Hkv, D, max_q, max_len) != AXHIP_OK) return 0;
   if (max_q > tokens) max_q = tokens;
-  const Sizes z = sizes_for(tile_rows_of(dtype, D), tokens, B, Hkv, Hq / Hkv, max_q, max_len);
+  const Sizes z = sizes_for(tile_of(dtype, D), tokens, B, Hkv, Hq / Hkv, max_q, max_len);
   return static_cast<size_t>(z.slots) * z.slot_rows * (D + 2) * sizeof(float);
 }
 
@@ -926,7 +941,7 @@ AXHIP_API int axhip_chunk_attention_paged(const void *q, const void *k_pool, con
     return AXHIP_INVALID_PTR;
   if (max_q > tokens) max_q = tokens;
   const int group = Hq / Hkv;
-  const Sizes z = sizes_for(tile_rows_of(dtype, D), tokens, B, Hkv, group, max_q, max_len);
+  const Sizes z = sizes_for(tile_of(dtype, D), tokens, B, Hkv, group, max_q, max_len);
   const size_t need = static_cast<size_t>(z.slots) * z.slot_rows * (D + 2) * sizeof(float);
   if (need && (!workspace || !aligned_to(workspace, 16))) return AXHIP_INVALID_PTR;
   if (workspace_bytes < need) return AXHIP_OUT_OF_MEMORY;
