@@ -50,16 +50,19 @@ struct ChunkArgs {
 
 template <typename T, int D>
 struct Cfg {
-  // Column tiles per wavefront, and the fewest units of 128 keys of a piece.  fp32 products take long enough for one
-  // column tile, and with half the rows in a tile and pieces of a single unit small batches spread over more workgroups
-  // (D = 64; before: 2 and 2): 3 ragged prompts of 200 tokens 17 us against 29, 16 decoding sequences at 2000 keys 29
-  // against 39; against that 4 x 1000 tokens at 2000 keys 321 us against 314, 4096 tokens of one prompt 254 against 220.
-  // fp16 is slower with pieces of one unit (512 tokens of one prompt 25 us against 23) and gains nothing from it.
+  // Column tiles per wavefront, the fewest units of 128 keys of a piece, and the workgroups per CU that the cut aims at.
+  // fp32 products take long enough for one column tile, and with half the rows in a tile and pieces of a single unit small
+  // batches spread over more workgroups (D = 64, against 2 tiles, 2 units, 2 workgroups): 3 ragged prompts of 200 tokens
+  // 17 us against 29, 16 decoding sequences at 2000 keys 26 against 39, 4096 tokens of one prompt 189 against 220.
+  // A third workgroup fits there only (registers): 189 us against 254 with two; four pieces per CU: 300 tokens at 6000
+  // keys 52 us against 42.  fp16 is slower with pieces of one unit (512 tokens of one prompt 25 us against 23) and gains
+  // nothing from three workgroups (D = 64: 4 x 1000 tokens 64 us against 62; D = 128 has registers for two).
   static constexpr int NT = D == 256 || sizeof(T) == 4 ? 1 : 2;
   static constexpr int MIN = sizeof(T) == 4 ? 1 : 2;
+  static constexpr int AIM = D == 64 && sizeof(T) == 4 ? 3 : 2;
   static constexpr int TR = kWavesWg * 16 * NT;                        // rows per tile
   static constexpr int FEW = 16 * NT;                                  // rows up to which wavefronts deal the keys
-  static constexpr int KS = (D == 256 || (sizeof(T) == 4 && D == 128)) ? 32 : 64;  // keys per stage
+  static constexpr int KS = D == 256 || sizeof(T) == 4 ? 32 : 64;  // keys per stage
   static constexpr int E = 16 / sizeof(T);                             // elements per 16-byte unit
   static constexpr int UPR = D / E;                                    // units per row
   static constexpr int SW = (UPR < 16 ? UPR : 16) - 1;                 // swizzle mask
@@ -846,13 +849,13 @@ struct Sizes {
   int slot_rows, target;
 };
 struct Tile {
-  int rows, min_units;
+  int rows, min_units, aim;
 };
 template <typename T>
 Tile tile_for(int D) {
-  if (D == 64) return {Cfg<T, 64>::TR, Cfg<T, 64>::MIN};
-  if (D == 128) return {Cfg<T, 128>::TR, Cfg<T, 128>::MIN};
-  return {Cfg<T, 256>::TR, Cfg<T, 256>::MIN};
+  if (D == 64) return {Cfg<T, 64>::TR, Cfg<T, 64>::MIN, Cfg<T, 64>::AIM};
+  if (D == 128) return {Cfg<T, 128>::TR, Cfg<T, 128>::MIN, Cfg<T, 128>::AIM};
+  return {Cfg<T, 256>::TR, Cfg<T, 256>::MIN, Cfg<T, 256>::AIM};
 }
 Tile tile_of(int dtype, int D) { return dtype == AXHIP_FLOAT32 ? tile_for<float>(D) : tile_for<__half>(D); }
 
@@ -866,7 +869,7 @@ Sizes sizes_for(Tile tile, int tokens, int B, int Hkv, int group, int max_q, int
   z.tiles = rows / tile_rows + B;
   const int64_t per_seq = (static_cast<int64_t>(max_q) * group + tile_rows - 1) / tile_rows;
   if (z.tiles > per_seq * B) z.tiles = per_seq * B;
-  z.target = 2 * device_cu_count();
+  z.target = tile.aim * device_cu_count();
   const int64_t units = (static_cast<int64_t>(max_len) + 127) / 128;
   const int64_t most = (units + tile.min_units - 1) / tile.min_units;  // pieces of one tile
   const int64_t cut = 4 * static_cast<int64_t>(z.target) / Hkv + 1;    // pieces of cut tiles, per kv head
