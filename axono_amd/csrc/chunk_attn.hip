@@ -21,8 +21,8 @@
 // an unnormalised state in the workspace; a second kernel adds the pieces of a tile in a fixed order.  No counters, no
 // state between launches: launches with workspaces of their own may overlap.
 //
-// fp32 statistics throughout.  fp16: probabilities are rounded to fp16 for the second product (2^-12 of their value at
-// most, random in sign), numerator and denominator from the same rounded values.  fp32: fp32 matrix instructions.
+// fp32 statistics throughout.  fp16: probabilities are rounded to fp16 for the second product (2^-11 of their value at
+// most; see softmax()), numerator and denominator from the same rounded values.  fp32: fp32 matrix instructions.
 #include "common.hpp"
 
 #include <type_traits>
@@ -34,6 +34,7 @@ constexpr int kThreads = 256;
 constexpr int kWavesWg = 4;
 constexpr int kPageKeys = 128, kPageShift = 7;
 constexpr int kBlockKeys = 32;      // keys of one softmax step
+constexpr int64_t kMostWorkgroups = (1 << 24) - 1;  // a launch has less than 2^32 threads
 constexpr float kMasked = -1.0e30f;
 typedef float float8_t __attribute__((ext_vector_type(8)));
 
@@ -143,6 +144,7 @@ __device__ __forceinline__ bool find_piece(const ChunkArgs &a, int flat, int lan
       const int l = __ffsll(static_cast<unsigned long long>(hit)) - 1;
       auto at = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
       const int rest = flat - at(upto - mine);
+      if (static_cast<unsigned>(rest) >= static_cast<unsigned>(at(mine))) return false;  // (sums past 31 bits: cu falls and rises)
       p.b = j + l;
       p.c0 = at(s.c0);
       p.start = at(s.start);
@@ -382,9 +384,12 @@ struct Wave {
         if (MASK && x <= kMasked) p[t][j] = 0.f;
       }
   }
-  // Probabilities against the running maximum as it stands: it is moved, and everything rescaled, only when one of them
-  // passes 2^8 (the first block of a row always does).  Until then p <= 256, which fp16 holds to the same 11 bits, and a
-  // block needs no maximum over its row at all.  (The maximum never runs ahead, so no p is smaller than against the true one.)
+  // Probabilities against a level that follows the running maximum: it is moved, and everything rescaled, only when one of
+  // them passes kTop (the first block of a row always does).  Until then a block needs no maximum over its row at all.
+  // fp16: the level lies 2^kBelow under the maximum that set it, so that p is 2^10 at the maximum and 2^15 at most: below
+  // 2^-24 of the largest weight of a row its others lose bits, below 2^-35 they are lost.  (Against the maximum itself those
+  // under 2^-25 would be, and 65536 such keys hold 2^-9 of the sum.)
+  static constexpr float kBelow = kHalf ? 10.f : 0.f, kTop = kHalf ? 32768.f : 256.f;
   // MASK: some key of the block at kb is behind some row's position.
   template <bool MASK>
   __device__ __forceinline__ void softmax(const float4_t (&sc)[NT][2], int kb, Probs (&pf)[NT]) {
@@ -395,13 +400,13 @@ struct Wave {
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = fmaxf(top, p[t][j]);
-    if (__builtin_expect(__any(top > 256.f), 0)) {
+    if (__builtin_expect(__any(top > kTop), 0)) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float mx = score<MASK>(sc, kb, t, 0);
 #pragma unroll
         for (int j = 1; j < 8; ++j) mx = fmaxf(mx, score<MASK>(sc, kb, t, j));
-        const float mnew = fmaxf(m[t], max_xor32(max_xor16(mx)) * a.scale_log2e);
+        const float mnew = fmaxf(m[t], max_xor32(max_xor16(mx)) * a.scale_log2e - kBelow);
         const float corr = __builtin_amdgcn_exp2f(m[t] - mnew);
         m[t] = mnew;
         lsum[t] *= corr;
@@ -751,7 +756,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
   int64_t part = -1;
   if (pc.pieces > 1) {
     const int64_t slot = static_cast<int64_t>(pc.slot) * a.Hkv + hk;
-    if (slot >= a.slots || n_rows > a.slot_rows) return;  // (cannot happen: the cut is bounded by both)
+    if (slot < 0 || slot >= a.slots || n_rows > a.slot_rows) return;  // (only where cu falls and rises: the cut is bounded by both)
     part = slot * a.slot_rows;
   }
   int *flag = reinterpret_cast<int *>(chunk_smem + C::kLdsBytes - 16);
@@ -797,7 +802,7 @@ __global__ __launch_bounds__(kMergeThreads) void chunk_merge_kernel(ChunkArgs a)
   Piece pc;
   if (!find_piece<C, true>(a, blockIdx.x / a.Hkv, tid & 63, pc)) return;
   const int row0 = pc.tile * C::TR, n_rows = min(pc.rows - row0, C::TR);
-  if ((static_cast<int64_t>(pc.slot) + pc.pieces - 1) * a.Hkv + hk >= a.slots || n_rows > a.slot_rows) return;
+  if (pc.slot < 0 || (static_cast<int64_t>(pc.slot) + pc.pieces - 1) * a.Hkv + hk >= a.slots || n_rows > a.slot_rows) return;
   constexpr int kAhead = 4;
   const int first = blockIdx.y * kMergeRows, rows = min(kMergeRows, n_rows - first);
   if (rows <= 0) return;
@@ -948,7 +953,7 @@ AXHIP_API int axhip_chunk_attention_paged(const void *q, const void *k_pool, con
   const size_t need = static_cast<size_t>(z.slots) * z.slot_rows * (D + 2) * sizeof(float);
   if (need && (!workspace || !aligned_to(workspace, 16))) return AXHIP_INVALID_PTR;
   if (workspace_bytes < need) return AXHIP_OUT_OF_MEMORY;
-  if (z.grid * Hkv > INT32_MAX) return AXHIP_INVALID_ARGUMENT;
+  if (z.grid * Hkv > kMostWorkgroups) return AXHIP_INVALID_ARGUMENT;
   ChunkArgs a{};
   a.q = q;
   a.k = k_pool;

@@ -177,3 +177,20 @@ def test_agrees_with_prefill_attention_of_the_dense_cache():
              "prefill_attention")
     _, tol = ps.chunk_want(q, k, v, table, [S], [0], S)
     assert np.all(np.abs(got.astype(float) - out.download(np.float16, q.shape).astype(float)) <= 2 * tol)
+
+
+def test_many_small_weights_add_up():
+    """A row whose first key has score 17.5 and its 65535 others 0: each of these weighs e^-17.5 = 2^-25.2, together 2^-9.2.  256 x 2
+    tiles over the same pages fill the device, so that most of a row's keys are taken in one piece.  The result is
+    N e^-17.5 / (1 + N e^-17.5) to the rounding of such a weight, 2^-25 / 2^-15.3 at 2^10 for the largest, and of the result."""
+    B, hk, keys = 256, 2, 65536
+    k, v = (np.zeros((keys // 128, hk, 128, 64), np.float16) for _ in range(2))
+    v[...] = 1
+    k[0, :, 0, 0], v[0, :, 0] = 17.5, 0
+    q = np.zeros((B, hk, 64), np.float16)
+    q[..., 0] = 8
+    table = np.tile(np.arange(keys // 128, dtype=np.int32), (B, 1))
+    got = ps.chunk(q, k, v, table, ps.cu_of([1] * B), [keys - 1] * B, 1, keys).astype(np.float64)
+    rest = (keys - 1) * np.exp(-17.5)
+    want = rest / (1 + rest)
+    assert np.abs(got / want - 1).max() <= 2.0 ** -9.7 + 2.0 ** -11 + 2.0 ** -17
