@@ -19,6 +19,7 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kAhead = 4;        // loads of a thread on their way at a time
 constexpr int kMostLds = 96 * 1024;
+constexpr int kMostBias = 16384;  // every biased token walks the list
 
 struct LogitsArgs {
   const void *x;
@@ -115,8 +116,7 @@ __global__ __launch_bounds__(kThreads) void logits_kernel(LogitsArgs a) {
   S *y = static_cast<S *>(a.out) + row * a.out_stride;
   const CT *words = reinterpret_cast<const CT *>(logits_smem);
   const uint32_t *allowed = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-  // Whole wavefronts stay in the loop: the search for a bias is
-  // theirs together.
+  // Whole wavefronts stay in the loop: the search for a bias is theirs together.
   for (int i0 = 0; i0 < n; i0 += kThreads * V * kAhead) {
     vec in[kAhead];
 #pragma unroll
@@ -214,7 +214,8 @@ AXHIP_API int axhip_logits_process(const void *logits, int64_t logits_stride, in
                                    axhip_stream stream) {
   if (!is_float_dtype(dtype)) return AXHIP_UNSUPPORTED_TYPE;
   if (history && history_dtype != AXHIP_INT32 && history_dtype != AXHIP_INT64) return AXHIP_UNSUPPORTED_TYPE;
-  if (rows < 0 || rows > 65535 || vocab < 0 || vocab > (1 << 30) || max_history < 0 || max_history >= (1 << 30) || bias_count < 0)
+  if (rows < 0 || rows > 65535 || vocab < 0 || vocab > (1 << 30) || max_history < 0 || max_history >= (1 << 30) || bias_count < 0 ||
+      bias_count > kMostBias)
     return AXHIP_INVALID_ARGUMENT;
   if (logits_stride < vocab || out_stride < vocab || history_row_stride < 0 || history_token_stride < 0) return AXHIP_INVALID_ARGUMENT;
   if (allowed && allowed_stride < (static_cast<int64_t>(vocab) + 31) / 32) return AXHIP_INVALID_ARGUMENT;

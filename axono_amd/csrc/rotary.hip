@@ -25,6 +25,7 @@ constexpr int kBlock = 256;
 constexpr int kWaves = kBlock / 64;
 constexpr int kMaxPairs = 256;   // rotary_dim <= 512
 constexpr int kPageShift = 7;    // 128 keys per page
+constexpr int64_t kMostRows = int64_t(1) << 25;  // of a launch: 2^32 threads are too many
 
 struct RotaryArgs {
   const void *x[3];       // q, k, v rows
@@ -36,7 +37,7 @@ struct RotaryArgs {
   const void *w[2];       // norm weights of q and k heads [D] or null
   int w_f16, norm;
   float eps, scale;
-  int64_t rows;
+  int64_t first, end, rows;  // rows of this launch; all rows
   int dim, rotary_dim, interleaved, axes, h_lim, w_lim;
   int lanes_shift;        // log2 of the lanes a head is spread over
   int groups, heads_per_group;
@@ -99,9 +100,9 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
   __shared__ float s_cos[kWaves][kMaxPairs], s_sin[kWaves][kMaxPairs];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * kWaves + wave;
-  const int64_t t = unit / a.groups;
-  if (t >= a.rows) return;  // whole wavefronts leave; nothing below waits for another wavefront
-  const int group = static_cast<int>(unit - t * a.groups);
+  const int64_t t = a.first + unit / a.groups;
+  if (t >= a.end) return;  // whole wavefronts leave; nothing below waits for another wavefront
+  const int group = static_cast<int>(unit % a.groups);
 
   int64_t cache_row = -1, cache_pos = t;  // element offset / D of head 0 of the token's row in its page; -1: not stored
   if constexpr (PAGED) {
@@ -313,25 +314,27 @@ int launch(RotaryArgs a, hipStream_t st) {
   if (per > rounds) per = rounds;
   a.heads_per_group = static_cast<int>(per) * step;
   a.groups = (all + a.heads_per_group - 1) / a.heads_per_group;
-  const int64_t grid = (a.rows * a.groups + kWaves - 1) / kWaves;
-  if (grid > INT32_MAX) return AXHIP_INVALID_ARGUMENT;
-  const dim3 g(static_cast<unsigned>(grid)), b(kBlock);
   // Results that would push the input of the next operators out of the 256 MB memory-side cache are stored past it (33001 rows
   // in fp32 150 -> 135 us, 65536 rows into the pages 317 -> 286 us); smaller ones are about to be read again.
+  const bool stream = a.rows * all * a.dim * static_cast<int64_t>(sizeof(TO)) >= (int64_t(64) << 20);
   constexpr int kWide = 16 / sizeof(TI);
-  if (v == kWide) {
-    if (a.rows * all * a.dim * static_cast<int64_t>(sizeof(TO)) >= (int64_t(64) << 20))
-      hipLaunchKernelGGL((rotary_kernel<TI, TO, kWide, 1, PAGED, true>), g, b, 0, st, a);
-    else
-      hipLaunchKernelGGL((rotary_kernel<TI, TO, kWide, 1, PAGED>), g, b, 0, st, a);
-  } else if (v == 4) {
-    if constexpr (kWide > 4) hipLaunchKernelGGL((rotary_kernel<TI, TO, 4, 1, PAGED>), g, b, 0, st, a);
-  } else if (v == 2) {
-    hipLaunchKernelGGL((rotary_kernel<TI, TO, 2, 2, PAGED>), g, b, 0, st, a);
-  } else {
-    hipLaunchKernelGGL((rotary_kernel<TI, TO, 1, 4, PAGED>), g, b, 0, st, a);
+  for (a.first = 0; a.first < a.rows; a.first = a.end) {
+    a.end = a.rows - a.first < kMostRows ? a.rows : a.first + kMostRows;  // (that many only where a.groups is 1)
+    const dim3 g(static_cast<unsigned>(((a.end - a.first) * a.groups + kWaves - 1) / kWaves)), b(kBlock);
+    if (v == kWide) {
+      if (stream) hipLaunchKernelGGL((rotary_kernel<TI, TO, kWide, 1, PAGED, true>), g, b, 0, st, a);
+      else hipLaunchKernelGGL((rotary_kernel<TI, TO, kWide, 1, PAGED>), g, b, 0, st, a);
+    } else if (v == 4) {
+      if constexpr (kWide > 4) hipLaunchKernelGGL((rotary_kernel<TI, TO, 4, 1, PAGED>), g, b, 0, st, a);
+    } else if (v == 2) {
+      hipLaunchKernelGGL((rotary_kernel<TI, TO, 2, 2, PAGED>), g, b, 0, st, a);
+    } else {
+      hipLaunchKernelGGL((rotary_kernel<TI, TO, 1, 4, PAGED>), g, b, 0, st, a);
+    }
+    const int rc = launch_status();
+    if (rc != AXHIP_OK) return rc;
   }
-  return launch_status();
+  return AXHIP_OK;
 }
 
 bool aligned_to(const void *p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -378,6 +381,9 @@ AXHIP_API int axhip_rotary_qk(const void *q, int64_t q_stride, const void *k, in
   if (rows > INT32_MAX) return AXHIP_INVALID_ARGUMENT;
   if ((q_heads && q_stride < static_cast<int64_t>(q_heads) * dim) || (k_heads && k_stride < static_cast<int64_t>(k_heads) * dim))
     return AXHIP_INVALID_ARGUMENT;
+  if ((q_heads && q == q_out && q_stride != static_cast<int64_t>(q_heads) * dim) ||
+      (k_heads && k == k_out && k_stride != static_cast<int64_t>(k_heads) * dim))
+    return AXHIP_INVALID_ARGUMENT;  // results would be written over rows that are still to be read
   if (rows == 0 || q_heads + k_heads == 0) return AXHIP_OK;
   if (!pos || !inv_freq || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out))) return AXHIP_INVALID_PTR;
   const int esz = dtype == AXHIP_FLOAT16 ? 2 : 4;
@@ -416,7 +422,7 @@ AXHIP_API int axhip_rotary_append_paged(const void *q, int64_t q_stride, const v
   if (!is_float_dtype(dtype) || !is_float_dtype(cache_dtype)) return AXHIP_UNSUPPORTED_TYPE;
   if (norm && (q_weight || k_weight) && !is_float_dtype(w_dtype)) return AXHIP_UNSUPPORTED_TYPE;
   if (tokens < 0 || B < 0 || Hq <= 0 || Hkv <= 0 || max_pages <= 0 || n_pages <= 0) return AXHIP_INVALID_ARGUMENT;
-  if (Hq > 32767 || Hkv > 16383) return AXHIP_INVALID_ARGUMENT;
+  if (Hq > 32767 || Hkv > 16383 || B > (1 << 20)) return AXHIP_INVALID_ARGUMENT;
   if (D <= 0 || D > 512 || D % 8 != 0 || rotary_dim <= 0 || rotary_dim % 2 != 0 || rotary_dim > D) return AXHIP_INVALID_ARGUMENT;
   if (pos_axes != 1 && pos_axes != 3) return AXHIP_INVALID_ARGUMENT;
   if (!pos && pos_axes != 1) return AXHIP_INVALID_ARGUMENT;

@@ -318,8 +318,11 @@ class PagedKVCache(KVCache):
                                         max(min(bound, self.max_len), 1), workspace=workspace)
 
     def advance_each(self, new_tokens) -> None:
-        """Sequence b grew by new_tokens[b] (after the last layer of a ragged batch)."""
-        self._lens += np.asarray(new_tokens, np.int64).reshape(self.batch)
+        """Sequence b grew by new_tokens[b] (after the last layer of a ragged batch, whose pages were reserved)."""
+        grown = np.asarray(new_tokens, np.int64).reshape(self.batch)
+        if np.any(grown < 0) or np.any((self._lens + grown + self.PAGE - 1) // self.PAGE > self._owned):
+            raise ValueError("PagedKVCache.advance_each: a negative number of tokens, or a sequence with fewer pages than they need")
+        self._lens += grown
         self.seq_lens.copy_from_numpy(self._lens.astype(np.int32))
 
     def set_lengths(self, lens) -> None:

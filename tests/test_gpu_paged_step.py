@@ -214,3 +214,14 @@ def test_surface_functions_and_their_refusals():
         L.rotary_inv_freq(32, kind="other")
     with pytest.raises(ValueError):
         decoders(1, 128)[0].prefill_chunk([[1], [2]])
+
+
+def test_advance_each_needs_the_pages():
+    cache = nn.PagedKVCache(1, 2, 1, 64, 6, 512, device="hip:0")
+    cache.reserve([100, 300])
+    cache.advance_each([100, 300])
+    for bad in ([29, 0], [0, 85], [-1, 0]):
+        with pytest.raises(ValueError):
+            cache.advance_each(bad)
+    cache.advance_each([28, 84])
+    assert cache.seq_lens.to_numpy().tolist() == [128, 384]

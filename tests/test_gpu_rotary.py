@@ -91,6 +91,18 @@ def test_rotary_in_place_and_special_values():
                      np.where(np.isfinite(size), size, 0) * ps.ROTATION + np.where(np.isfinite(want), np.abs(want), 0) * 2.0 ** -24)
 
 
+def test_more_rows_than_one_launch_takes():
+    rows = (1 << 25) + 70
+    x = np.tile(np.arange(1, 57, dtype=np.float16).reshape(7, 1, 8) / 8, (rows // 7 + 1, 1, 1))[:rows]
+    pos, f = np.arange(rows, dtype=np.int64) % 1000, table(8)
+    dx, dp, df = ps.dev(x), ps.dev(pos), ps.dev(f)
+    ps.check(ps.lib().axhip_rotary_qk(dx.ptr, 8, None, 0, dp.ptr, df.ptr, 1.0, 0, 8, dx.ptr, None, ps.F16, rows, 1, 0, 8, None), "rotary_qk")
+    got = dx.download(np.float16, x.shape)
+    for at in (slice(0, 200), slice((1 << 25) - 100, rows)):
+        want, size = ps.turned(x[at], pos[at], f, 8, False, 1.0)
+        ps.assert_within(got[at], want, size * ps.ROTATION + np.abs(want) * 2.0 ** -11 + 2.0 ** -25)
+
+
 # ---- append ------------------------------------------------------------------------------------------------------------
 CASES = [
     # n, start, hq, hk, d, rd, interleaved, norm, axes

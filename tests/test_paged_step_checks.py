@@ -164,3 +164,11 @@ def test_host_tensors_are_refused():
         assert e.value.code == Status.DEVICE_MISMATCH
     table, scale = L.rotary_inv_freq(64, 1e4, "linear", factor=2.0, device="cpu")
     assert scale == 1.0 and table.shape == [32] and abs(float(table.to_numpy()[0]) - 0.5) < 1e-7
+
+
+def test_sizes_that_no_launch_takes_are_refused():
+    # in place with gaps between the rows: a row's result would land on rows that are still to be read
+    assert rotary(rows=2, qs=192, qo=P) == INVALID and rotary(rows=2, ks=128, qo=P + 4096, ko=P) == INVALID
+    assert append(B=(1 << 20) + 1) == INVALID
+    assert chunk(T=1 << 20, B=1 << 20, hq=32, hk=32) == INVALID          # 2^25 workgroups
+    assert logits(rows=1, bc=16385) == INVALID
