@@ -225,3 +225,31 @@ def test_advance_each_needs_the_pages():
             cache.advance_each(bad)
     cache.advance_each([28, 84])
     assert cache.seq_lens.to_numpy().tolist() == [128, 384]
+
+
+def test_pages_beyond_four_gigabytes():
+    """the same pages at the end of a pool of 4.3 GB and in a small one: the same bits"""
+    hq, hk, d, far = 8, 8, 128, 16500
+    rng = np.random.default_rng(11)
+    n, start, where = [3, 1], [254, 5], [far - 1, 7, 16390, far - 3]
+    near_table = np.array([[0, 1, 2], [3, -1, -1]], np.int32)
+    far_table = np.array([where[:3], [where[3], -1, -1]], np.int32)
+    page_bytes = hk * 128 * d * 2
+    table, _ = L.rotary_inv_freq(d, 1e6, device="hip:0")
+    cu, st = hip(ps.cu_of(n)), hip(np.array(start, np.int32))
+    qkv = hip(rng.standard_normal((4, (hq + 2 * hk) * d)).astype(np.float32))
+    old = [hip(rng.standard_normal((4, hk, 128, d)).astype(np.float16)) for _ in range(2)]
+    pools = [Tensor(DataType.FLOAT16, [far, hk, 128, d], "hip:0", _zero=False) for _ in range(2)]
+    for small, large in zip(old, pools):
+        for i, p in enumerate(where):
+            L.copy_bytes(large, p * page_bytes, small, i * page_bytes, page_bytes)
+    results = []
+    for ks, tb in ((old, near_table), (pools, far_table)):
+        q = L.rotary_append_paged(qkv, hq, table, cu, st, *ks, hip(tb), eps=1e-6)
+        results.append(L.chunk_attention_paged(q, *ks, hip(tb), cu, st, 3, 257).to_numpy())
+    np.testing.assert_array_equal(results[0], results[1])
+    for small, large in zip(old, pools):
+        back = Tensor(DataType.FLOAT16, [4, hk, 128, d], "hip:0")
+        for i, p in enumerate(where):
+            L.copy_bytes(back, i * page_bytes, large, p * page_bytes, page_bytes)
+        np.testing.assert_array_equal(back.to_numpy(), small.to_numpy())
