@@ -46,6 +46,7 @@ struct ChunkArgs {
   float *part_ml;  // [slots][slot_rows][2]: maximum (log2 units), sum
   int tokens, B, Hq, Hkv, group, max_q, max_len, max_pages, n_pages;
   int slots, slot_rows, target;  // target: pieces the launch aims at
+  int merge_rows;                // rows per workgroup of the merge
   float scale_log2e;
 };
 
@@ -779,7 +780,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
   }
 }
 
-// Adds the pieces of a cut tile: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  A workgroup takes 16 rows of the tile;
+// Adds the pieces of a cut tile: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  A workgroup takes up to 16 rows of the tile;
 // where these are fewer, or the pieces many, several threads share an element and take every P-th piece each, and their sums
 // are added up in order through LDS: a thread has four pieces on their way at a time, and what bounds this kernel is the
 // chain of such trips (one row of 128 pieces: 8 trips instead of 32).
@@ -804,7 +805,7 @@ __global__ __launch_bounds__(kMergeThreads) void chunk_merge_kernel(ChunkArgs a)
   const int row0 = pc.tile * C::TR, n_rows = min(pc.rows - row0, C::TR);
   if (pc.slot < 0 || (static_cast<int64_t>(pc.slot) + pc.pieces - 1) * a.Hkv + hk >= a.slots || n_rows > a.slot_rows) return;
   constexpr int kAhead = 4;
-  const int first = blockIdx.y * kMergeRows, rows = min(kMergeRows, n_rows - first);
+  const int first = blockIdx.y * a.merge_rows, rows = min(a.merge_rows, n_rows - first);
   if (rows <= 0) return;
   const int64_t step = static_cast<int64_t>(a.Hkv) * a.slot_rows;  // between the pieces' states
   // threads of an element: a power of two, all of them with the same piece in neighbouring threads
@@ -891,17 +892,26 @@ Sizes sizes_for(Tile tile, int tokens, int B, int Hkv, int group, int max_q, int
   return z;
 }
 template <typename T, int D>
-int launch(const ChunkArgs &a, const Sizes &z, hipStream_t st) {
+int launch(ChunkArgs a, const Sizes &z, hipStream_t st) {
   using C = Cfg<T, D>;
   static std::atomic<uint64_t> raised{0};
   const int rc = raise_dynamic_lds(reinterpret_cast<const void *>(&chunk_attn_kernel<T, D>), C::kLdsBytes, raised);
   if (rc != AXHIP_OK) return rc;
   hipLaunchKernelGGL((chunk_attn_kernel<T, D>), dim3(static_cast<unsigned>(z.grid * a.Hkv)), dim3(kThreads), C::kLdsBytes, st, a);
   if (z.cut_tiles > 0) {
-    // 1024 threads where every tile has few rows (1 row of 32768 keys: 40 us against 51), 256 where most workgroups find
-    // sixteen rows of few pieces or none (8 x 2000 rows: 109 us against 123)
-    const dim3 grid(static_cast<unsigned>(z.cut_tiles * a.Hkv), (z.slot_rows + kMergeRows - 1) / kMergeRows);
-    if (z.slot_rows <= kMergeRows) hipLaunchKernelGGL((chunk_merge_kernel<T, D, 1024>), grid, dim3(1024), 0, st, a);
+    // 1024 threads where every tile has few rows or there are few tiles (1 row of 32768 keys: 40 us against 51), 256 where most
+    // workgroups find sixteen rows of few pieces or none (8 x 2000 rows: 109 us against 123).  Fewer rows a workgroup, and
+    // more threads an element, as long as that leaves a workgroup per CU (16 heads of one token over 128000 keys 35 us, 123 us
+    // with 16 rows; 64 tokens at 16000 keys 33 us against 61), of 256 threads four (512 tokens at 8000 keys 60 us against 63;
+    // 8 x 2000 tokens 205 us with 8 rows, 200 us with 16).
+    const int cus = device_cu_count(), tiles = static_cast<int>(z.cut_tiles * a.Hkv);
+    const auto groups = [&](int rows) { return (z.slot_rows + rows - 1) / rows; };
+    const bool wide = groups(kMergeRows) == 1 || tiles * groups(kMergeRows) <= cus;
+    const int most = wide ? cus : 4 * cus;
+    a.merge_rows = kMergeRows;
+    while (a.merge_rows > 1 && tiles * groups(a.merge_rows / 2) <= most) a.merge_rows /= 2;
+    const dim3 grid(static_cast<unsigned>(tiles), groups(a.merge_rows));
+    if (wide) hipLaunchKernelGGL((chunk_merge_kernel<T, D, 1024>), grid, dim3(1024), 0, st, a);
     else hipLaunchKernelGGL((chunk_merge_kernel<T, D, 256>), grid, dim3(256), 0, st, a);
   }
   return launch_status();
