@@ -784,7 +784,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
 
 // Adds the pieces of a cut tile: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  A workgroup takes up to 16 rows of the tile;
 // where these are fewer, or the pieces many, several threads share an element and take every P-th piece each, and their sums
-// are added up in order through LDS: a thread has four pieces on their way at a time, and what bounds this kernel is the
+// are added up in a fixed tree through LDS (one row of 63 pieces: 5.6 us, 8.4 us one after the other): a thread has four pieces on their way at a time, and what bounds this kernel is the
 // chain of such trips (one row of 128 pieces: 8 trips instead of 32).
 constexpr int kMergeRows = 16;
 struct Sum {
@@ -834,13 +834,14 @@ __global__ __launch_bounds__(kMergeThreads) void chunk_merge_kernel(ChunkArgs a)
         if (s0 + i * parts < pc.pieces) add_sum(sum, got[i]);
     }
   }
+  // (parts is a power of two, like all the sizes it is made from; one that had no piece adds nothing)
   __shared__ Sum sums[kMergeThreads];
-  if (parts > 1) {
-    sums[tid] = sum;
+  for (int half = parts / 2; half > 0; half /= 2) {
+    if (part >= half && part < 2 * half) sums[tid] = sum;
     __syncthreads();
+    if (part < half) add_sum(sum, sums[tid + half * items]);
   }
   if (part > 0 || !live) continue;
-  for (int q = 1; q < min(parts, pc.pieces); ++q) add_sum(sum, sums[q * items + item]);
   const float inv = sum.l > 0.f ? 1.0f / sum.l : (sum.l == 0.f ? 0.f : sum.l);
   const int rr = row0 + r, i = rr / a.group;
   T *out = static_cast<T *>(a.out) + (static_cast<int64_t>(pc.c0 + i) * a.Hq + hk * a.group + (rr - i * a.group)) * D + d;
@@ -903,7 +904,7 @@ int launch(ChunkArgs a, const Sizes &z, hipStream_t st) {
   if (z.cut_tiles > 0) {
     // 1024 threads where every tile has few rows or there are few tiles (1 row of 32768 keys: 40 us against 51), 256 where most
     // workgroups find sixteen rows of few pieces or none (8 x 2000 rows: 109 us against 123).  Fewer rows a workgroup, and
-    // more threads an element, as long as that leaves a workgroup per CU (16 heads of one token over 128000 keys 35 us, 123 us
+    // more threads an element, as long as that leaves a workgroup per CU (16 heads of one token over 128000 keys 31 us, 120 us
     // with 16 rows; 64 tokens at 16000 keys 33 us against 61), of 256 threads four (512 tokens at 8000 keys 60 us against 63;
     // 8 x 2000 tokens 205 us with 8 rows, 200 us with 16).
     const int cus = device_cu_count(), tiles = static_cast<int>(z.cut_tiles * a.Hkv);
