@@ -233,6 +233,10 @@ struct Wave {
   static constexpr int NT = C::NT, KS = C::KS, UPR = C::UPR, SW = C::SW, DT = D / 16;
   static constexpr int QF = kHalf ? D / 32 : D / 4;  // operand registers of a column tile (8 halves or 1 float each)
   static constexpr int kRow = D * static_cast<int>(sizeof(T)), kTensor = 2 * KS * kRow;  // bytes: a row, both stages of K
+  // A row's 16-byte units lie XORed by these, so that the lanes of a read find 256 bytes of different banks: the same unit of 16
+  // rows of K; a pair of units of 8 rows of V.  Linear in the row's bits.
+  static constexpr __host__ __device__ int swz_k(int row) { return kHalf && D == 64 ? (row >> 1) & SW : row & SW; }
+  static constexpr __host__ __device__ int swz_v(int row) { return !kHalf ? row & SW : (D == 64 ? row & 6 : (2 * row) & 14); }
 
   const ChunkArgs &a;
   const Piece &pc;
@@ -281,9 +285,9 @@ struct Wave {
     vbase = static_cast<const T *>(a.v) + static_cast<int64_t>(hk) * kPageKeys * D;
     // Where this lane reads its operands, as byte offsets into a stage of K / V; the steps of the products flip or add constant
     // bits of them.  Made opaque where they are used, or the compiler keeps every one of the flipped offsets in registers.
-    kaddr = c * kRow + (kHalf ? (g ^ (c & SW)) * 16 : (c & SW) * 16 + g * 4);
+    kaddr = c * kRow + (kHalf ? (g ^ swz_k(c)) * 16 : swz_k(c) * 16 + g * 4);
     const int vkey = kHalf ? 4 * g + (c >> 2) : 4 * g;
-    vaddr = vkey * kRow + (kHalf ? ((((c & 3) >> 1) ^ (vkey & SW)) * 16 + (c & 1) * 8) : (((c >> 2) ^ (vkey & SW)) * 16 + (c & 3) * 4));
+    vaddr = vkey * kRow + (kHalf ? ((((c & 3) >> 1) ^ swz_v(vkey)) * 16 + (c & 1) * 8) : (((c >> 2) ^ swz_v(vkey)) * 16 + (c & 3) * 4));
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       m[t] = kMasked;
@@ -464,18 +468,18 @@ struct Wave {
 
   // ---- the keys in stages that the workgroup shares -------------------------------------------------------------------------
   // K and V go from memory to LDS directly (16 bytes a lane; a wavefront fills 1 KiB in lane order, so the swizzle is made on
-  // the side of memory: the lane of place u of a row fetches unit u ^ (row & SW)).  Load p of a thread covers row
+  // the side of memory: the lane of place u of a row fetches unit u ^ swz(row)).  Load p of a thread covers row
   // p kStep + tid / UPR of the stage; its offset within the page differs by constants from load 0's.
   static constexpr int kStep = kThreads / UPR;
   __device__ __forceinline__ void load_stage(int page, int key0, int buf) const {
     const int64_t base = key_at(page, key0);
     const unsigned place = buf * (KS * kRow) + wave * 1024;
-    const unsigned voff = tid / UPR * kRow + ((tid % UPR) ^ ((tid / UPR) & SW)) * 16;
+    const unsigned koff = tid / UPR * kRow + ((tid % UPR) ^ swz_k(tid / UPR)) * 16;
+    const unsigned voff = tid / UPR * kRow + ((tid % UPR) ^ swz_v(tid / UPR)) * 16;
 #pragma unroll
     for (int p = 0; p < C::VEC; ++p) {
-      const unsigned off = (voff ^ ((p * kStep & SW) * 16)) + p * kStep * kRow;
-      load_lds16(kbase + base, off, smem + place + p * kThreads * 16);
-      load_lds16(vbase + base, off, smem + kTensor + place + p * kThreads * 16);
+      load_lds16(kbase + base, (koff ^ (swz_k(p * kStep) * 16)) + p * kStep * kRow, smem + place + p * kThreads * 16);
+      load_lds16(vbase + base, (voff ^ (swz_v(p * kStep) * 16)) + p * kStep * kRow, smem + kTensor + place + p * kThreads * 16);
     }
   }
   // The units that this thread has fetched are in LDS, and clean.  (The barrier behind this call makes them everybody's.)
@@ -587,10 +591,10 @@ struct Wave {
     const int64_t base = key_at(page, kb);
     int l = lane;
     asm volatile("" : "+v"(l));  // offsets are made here, not kept
-    const unsigned v_row = static_cast<unsigned>(l) / UPR, v_off = v_row * kRow + ((l % UPR) ^ (v_row & SW)) * 16;
+    const unsigned v_row = static_cast<unsigned>(l) / UPR, v_off = v_row * kRow + ((l % UPR) ^ swz_v(v_row)) * 16;
 #pragma unroll
     for (int p = 0; p < kLoads; ++p)
-      load_lds16<T, 2>(vbase + base, (v_off ^ ((p * kRowsALoad & SW) * 16)) + p * 1024, smem + (wave * 2 + buf) * kVBytes + p * 1024);
+      load_lds16<T, 2>(vbase + base, (v_off ^ (swz_v(p * kRowsALoad) * 16)) + p * 1024, smem + (wave * 2 + buf) * kVBytes + p * 1024);
     const T *rows = kbase + base + (l & 15) * D + (l >> 4) * 8;
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk)
