@@ -6,8 +6,8 @@
 // n G "rows" per kv head, row r = (token r / G, head r % G): any G, and positions that grow with r.  A workgroup of four
 // wavefronts takes a tile of up to 64 NT rows of one (sequence, kv head) and a piece of the keys they see; a wavefront
 // takes NT column tiles of 16 rows.  In a tile with few rows (at most 16 NT: decoding sequences, drafts, the last rows of
-// a chunk) all wavefronts take the same rows and deal the 32-key blocks of a stage among themselves; their states are
-// added up at the end.
+// a chunk) all wavefronts take the same rows and deal the keys among themselves in blocks of 32; their states are added up at
+// the end.
 //
 // Everything is computed transposed, so that no operand changes its layout in registers (see the products below):
 //   S^T = K . Q^T  (16 keys x 16 rows), O^T += V^T . P^T  (16 d x 16 rows); a lane owns the row lane % 16 in both.
@@ -16,10 +16,15 @@
 // address of a stage is inside the pool whatever the lengths are.
 //
 // Few tiles over many keys would leave the device idle: the keys of a tile are cut into pieces so that the launch has
-// about two workgroups per CU of equal work.  The cut is made on the device from cu_tokens and start (every workgroup
+// about two workgroups per CU (fp32 with D = 64: three) of equal work.  The cut is made on the device from cu_tokens and start (every workgroup
 // derives it with a few wave operations), so a captured launch follows lengths that change.  A piece of a cut tile leaves
 // an unnormalised state in the workspace; a second kernel adds the pieces of a tile in a fixed order.  No counters, no
 // state between launches: launches with workspaces of their own may overlap.
+//
+// What bounds it, fp16 D = 128: from about 32 rows of a kv head on the matrix cores beside the exponentials (16 x 4096 tokens 1150 us =
+// 955 TFLOP/s, 2048 tokens at 129024 keys 1985 us = 1095 TFLOP/s, where a large library product reaches 1144); below that the
+// stream of keys (4 tokens each of 32 sequences, 573 MB: 6.0 TB/s, with the merge 111 us) and, where there are few keys too, the
+// plan, the merge and the two launches (about 5 us).
 //
 // fp32 statistics throughout.  fp16: probabilities are rounded to fp16 for the second product (2^-11 of their value at
 // most; see softmax()), numerator and denominator from the same rounded values.  fp32: fp32 matrix instructions.
