@@ -290,9 +290,9 @@ struct Wave {
     vbase = static_cast<const T *>(a.v) + static_cast<int64_t>(hk) * kPageKeys * D;
     // Where this lane reads its operands, as byte offsets into a stage of K / V; the steps of the products flip or add constant
     // bits of them.  Made opaque where they are used, or the compiler keeps every one of the flipped offsets in registers.
-    kaddr = c * kRow + (kHalf ? (g ^ swz_k(c)) * 16 : swz_k(c) * 16 + g * 4);
+    kaddr = c * kRow + (g ^ swz_k(c)) * 16;
     const int vkey = kHalf ? 4 * g + (c >> 2) : 4 * g;
-    vaddr = vkey * kRow + (kHalf ? ((((c & 3) >> 1) ^ swz_v(vkey)) * 16 + (c & 1) * 8) : (((c >> 2) ^ swz_v(vkey)) * 16 + (c & 3) * 4));
+    vaddr = vkey * kRow + (kHalf ? ((((c & 3) >> 1) ^ swz_v(vkey)) * 16 + (c & 1) * 8) : (c ^ swz_v(vkey)) * 16);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       m[t] = kMasked;
@@ -312,15 +312,21 @@ struct Wave {
     return min(max(page, 0), a.n_pages - 1) * page_elems + static_cast<int64_t>(key & (kPageKeys - 1)) * D;
   }
 
-  // Q as the right operand of the first product, for the whole piece
+  // Q as the right operand of the first product, for the whole piece.  fp32: product step 4 i + e takes d = 16 i + 4 g + e, so that a
+  // lane's operands of four steps are one 16-byte unit, of Q as of K.
   __device__ __forceinline__ void load_q() {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const S *qrow = static_cast<const S *>(a.q) + row_at(min(wrow + t * 16 + c, n_rows - 1));
 #pragma unroll
-      for (int kk = 0; kk < QF; ++kk) {
-        if constexpr (kHalf) qf[t][kk] = *reinterpret_cast<const half8_t *>(qrow + kk * 32 + g * 8);
-        else qf[t][kk] = qrow[kk * 4 + g];
+      for (int i = 0; i < D * static_cast<int>(sizeof(T)) / 64; ++i) {
+        if constexpr (kHalf) {
+          qf[t][i] = *reinterpret_cast<const half8_t *>(qrow + i * 32 + g * 8);
+        } else {
+          const float4_t x = *reinterpret_cast<const float4_t *>(qrow + i * 16 + g * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qf[t][4 * i + e] = x[e];
+        }
       }
     }
   }
@@ -348,25 +354,45 @@ struct Wave {
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk)
 #pragma unroll
-      for (int kk = 0; kk < QF; ++kk) kf[tk][kk] = lds_at<KFrag>(smem, (ka ^ (kk * (kHalf ? 64 : 16))) + tk * 16 * kRow);
+      for (int i = 0; i < kRow / 64; ++i) {
+        if constexpr (kHalf) {
+          kf[tk][i] = lds_at<KFrag>(smem, (ka ^ (i * 64)) + tk * 16 * kRow);
+        } else {
+          const float4_t x = lds_at<float4_t>(smem, (ka ^ (i * 64)) + tk * 16 * kRow);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) kf[tk][4 * i + e] = x[e];
+        }
+      }
   }
   // V^T fragments of a block, d tile by d tile.  fp32: product step (tk, e) takes keys tk * 16 + 4 g + e, g = 0 .. 3, so that
-  // a lane's score register e is its right operand.
+  // a lane's score register e is its right operand; d tile 4 h + i holds d = 64 h + 4 c + i, so that a lane's operands of four
+  // tiles are one 16-byte unit (single floats in their place: 3 x 819 tokens at 17600 keys, D = 128, 332 us against 298).
   __device__ __forceinline__ void read_v(int place, VFrag (&vf)[DT]) const {
     int va = vaddr + place;
     asm volatile("" : "+v"(va));
+    if constexpr (kHalf) {
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      if constexpr (kHalf) {
+      for (int dt = 0; dt < DT; ++dt) {
         const half4_t lo = lds_tr(smem, va ^ (dt * 32)), hi = lds_tr(smem, (va ^ (dt * 32)) + 16 * kRow);
         vf[dt] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          vf[dt][j] = lds_at<float>(smem, (va ^ (dt * 64) ^ ((j & 3) * 16)) + ((j >> 2) * 16 + (j & 3)) * kRow);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int h = 0; h < DT / 4; ++h) {
+          const float4_t x = lds_at<float4_t>(smem, (va ^ ((j & 3) * 16)) + ((j >> 2) * 16 + (j & 3)) * kRow + h * 256);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vf[4 * h + i][j] = x[i];
+        }
     }
   }
+  // Four results of this lane that lie side by side in a row, and where: n counts them, n < DT.
+  __device__ __forceinline__ float4_t four(int t, int n) const {
+    if constexpr (kHalf) return o[t][n];
+    else return float4_t{o[t][n & ~3][n & 3], o[t][(n & ~3) + 1][n & 3], o[t][(n & ~3) + 2][n & 3], o[t][(n & ~3) + 3][n & 3]};
+  }
+  __device__ __forceinline__ int four_at(int n) const { return kHalf ? n * 16 + 4 * g : (n >> 2) * 64 + 16 * g + 4 * (n & 3); }
   __device__ __forceinline__ void scores(const KFrag (&kf)[2][QF], float4_t (&sc)[NT][2]) const {
 #pragma unroll
     for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -529,7 +555,7 @@ struct Wave {
     // barrier that ends a stage stands in the middle of its last block, behind that block's last LDS read.
     // Of the two or three wavefronts of a SIMD the one at its products goes first: they fall out of step, and one's products run
     // under another's exponentials (2048 tokens at 129024 keys 2130 -> 1995 us, 16 x 4096 tokens 1188 -> 1151 us).
-    if constexpr (kHalf ? D <= 128 : D == 64) {  // (fp32 with D = 128: 4 x 512 rows 312 us this way, 288 us without)
+    if constexpr (!kHalf || D <= 128) {  // (fp32, D = 128: 4 x 512 tokens 80 us, 82 us without)
       const int seen = position(0) + 1 - k0;  // keys of the piece that all rows see
       const int n_fast = few || seen <= 0 ? 0 : min(seen / KS, n_stages);
       if (n_fast > 0) {
@@ -689,7 +715,7 @@ struct Wave {
       if (part >= 0) {
         float *po = a.part_o + (part + r) * D;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t *>(po + dt * 16 + 4 * g) = o[t][dt];
+        for (int n = 0; n < DT; ++n) *reinterpret_cast<float4_t *>(po + four_at(n)) = four(t, n);
         if (g == 0) {
           a.part_ml[(part + r) * 2] = m[t];
           a.part_ml[(part + r) * 2 + 1] = lsum[t][0];
@@ -698,12 +724,13 @@ struct Wave {
         const float inv = inverse(lsum[t][0]);
         S *orow = static_cast<S *>(a.out) + row_at(r);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
+        for (int n = 0; n < DT; ++n) {
           typedef S vec4 __attribute__((ext_vector_type(4)));
+          const float4_t x = four(t, n);
           vec4 h;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) h[e] = static_cast<S>(o[t][dt][e] * inv);
-          *reinterpret_cast<vec4 *>(orow + dt * 16 + 4 * g) = h;
+          for (int e = 0; e < 4; ++e) h[e] = static_cast<S>(x[e] * inv);
+          *reinterpret_cast<vec4 *>(orow + four_at(n)) = h;
         }
       }
     }
@@ -718,7 +745,7 @@ struct Wave {
       for (int t = 0; t < NT; ++t) {
         const int r = wave * C::FEW + t * 16 + c;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t *>(so + r * C::STATE + dt * 16 + 4 * g) = o[t][dt];
+        for (int n = 0; n < DT; ++n) *reinterpret_cast<float4_t *>(so + r * C::STATE + four_at(n)) = four(t, n);
         if (g == 0) {
           sml[2 * r] = m[t];
           sml[2 * r + 1] = lsum[t][0];
