@@ -74,7 +74,7 @@ struct Cfg {
   static constexpr int UPR = D / E;                                    // units per row
   static constexpr int SW = (UPR < 16 ? UPR : 16) - 1;                 // swizzle mask
   static constexpr int VEC = KS * UPR / kThreads;                      // units per thread, tensor and stage
-  static constexpr bool kOwnBlocks = sizeof(T) == 2 && D <= 128;       // see Wave::own_blocks
+  static constexpr bool kOwnBlocks = D <= 128;                         // see Wave::own_blocks
   static constexpr int STATE = D + 4;                                  // row stride of the states added up in LDS
   static constexpr int kStageBytes = 4 * KS * D * static_cast<int>(sizeof(T));
   // wavefronts with keys of their own in a tile of few rows
@@ -624,44 +624,66 @@ struct Wave {
     }
   }
 
-  // ---- few rows, fp16: every wavefront its own keys ---------------------------------------------------------------------------
+  // ---- few rows: every wavefront its own keys ---------------------------------------------------------------------------------
   // Bound by the stream of keys, so every wavefront takes blocks of its own (block i of the piece goes to wavefront i % 4) and
   // waits for nobody: K goes to registers in operand order (16 rows x 64 bytes a load), V through a strip of LDS of the
-  // wavefront's own, both a block ahead, read once and therefore past the caches.
+  // wavefront's own, both read once and therefore past the caches.
   static constexpr int kVBytes = kBlockKeys * kRow, kLoads = kVBytes / 1024;  // V of a block; loads of a lane for it, as many for K
-  __device__ __forceinline__ void fetch_own(int page, int kb, int buf, KFrag (&kf)[2][QF]) const {
+  static constexpr int kStrips = kHalf ? 2 : 1;                               // of a wavefront
+  __device__ __forceinline__ int strip_at(int buf) const { return (wave * kStrips + buf) * kVBytes; }
+  __device__ __forceinline__ void fetch_own_v(int page, int kb, int buf) const {
     constexpr int kRowsALoad = 1024 / kRow;
-    static_assert(2 * kWavesWg * kVBytes <= C::kStageBytes, "two blocks of V per wavefront fit the stages' LDS");
+    static_assert(!C::kOwnBlocks || kStrips * kWavesWg * kVBytes <= C::kStageBytes, "the strips fit the stages' LDS");
     const int64_t base = key_at(page, kb);
     int l = lane;
     asm volatile("" : "+v"(l));  // offsets are made here, not kept
     const unsigned v_row = static_cast<unsigned>(l) / UPR, v_off = v_row * kRow + ((l % UPR) ^ swz_v(v_row)) * 16;
 #pragma unroll
     for (int p = 0; p < kLoads; ++p)
-      load_lds16<T, 2>(vbase + base, (v_off ^ (swz_v(p * kRowsALoad) * 16)) + p * 1024, smem + (wave * 2 + buf) * kVBytes + p * 1024);
-    const T *rows = kbase + base + (l & 15) * D + (l >> 4) * 8;
+      load_lds16<T, 2>(vbase + base, (v_off ^ (swz_v(p * kRowsALoad) * 16)) + p * 1024, smem + strip_at(buf) + p * 1024);
+  }
+  __device__ __forceinline__ void fetch_own_k(int page, int kb, KFrag (&kf)[2][QF]) const {
+    constexpr int E = C::E;
+    const int64_t base = key_at(page, kb);
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    const T *rows = kbase + base + (l & 15) * D + (l >> 4) * E;
 #pragma unroll
     for (int tk = 0; tk < 2; ++tk)
 #pragma unroll
-      for (int kk = 0; kk < QF; ++kk)
-        kf[tk][kk] = __builtin_bit_cast(half8_t, __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(rows + tk * 16 * D + kk * 32)));
+      for (int i = 0; i < kRow / 64; ++i) {
+        const u32x4_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(rows + tk * 16 * D + i * 4 * E));
+        if constexpr (kHalf) {
+          kf[tk][i] = __builtin_bit_cast(half8_t, x);
+        } else {
+          const float4_t f = __builtin_bit_cast(float4_t, x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) kf[tk][4 * i + e] = f[e];
+        }
+      }
   }
-  __device__ __forceinline__ void use_own(int kb, int buf, const KFrag (&kf)[2][QF]) {
-    float4_t sc[NT][2];
-    Probs pf[NT];
-    scores(kf, sc);
-    __builtin_amdgcn_sched_barrier(0);
-    const int strip = (wave * 2 + buf) * kVBytes;
+  __device__ __forceinline__ void fetch_own(int page, int kb, int buf, KFrag (&kf)[2][QF]) const {
+    fetch_own_v(page, kb, buf);
+    fetch_own_k(page, kb, kf);
+  }
+  __device__ __forceinline__ void clean_own(int kb, int strip) const {
     if (kb + kBlockKeys > mixed_from) {
       bool bad = false;
 #pragma unroll 1
       for (int p = 0; p < kLoads; ++p) bad |= clean(smem + strip + p * 1024 + lane * 16, kb + (p * 64 + lane) / UPR);
       if (bad) *flag = 1;
     }
+  }
+  __device__ __forceinline__ void use_own(int kb, int buf, const KFrag (&kf)[2][QF]) {
+    float4_t sc[NT][2];
+    Probs pf[NT];
+    scores(kf, sc);
+    __builtin_amdgcn_sched_barrier(0);
+    clean_own(kb, strip_at(buf));
     softmax<true>(sc, kb, pf);
     __builtin_amdgcn_sched_barrier(0);
     VFrag vf[DT];
-    read_v(strip, vf);
+    read_v(strip_at(buf), vf);
     add_values(vf, pf);
   }
   __device__ __forceinline__ void own_blocks() {
@@ -673,6 +695,12 @@ struct Wave {
     int page = page_of(kb + kHop);
     load_q();
     asm volatile("" ::: "memory");  // the queries' loads are issued before the keys'
+    if constexpr (kHalf) own_two_ahead(kb, page0, page);
+    else own_one(kb, page0, page);
+  }
+  // fp16: both a block ahead.
+  __device__ __forceinline__ void own_two_ahead(int kb, int page0, int page) {
+    constexpr int kHop = kWavesWg * kBlockKeys;
     KFrag now[2][QF], next[2][QF];
     fetch_own(page0, kb, 0, now);
 #pragma unroll 1
@@ -693,6 +721,34 @@ struct Wave {
       for (int tk = 0; tk < 2; ++tk)
 #pragma unroll
         for (int kk = 0; kk < QF; ++kk) now[tk][kk] = next[tk][kk];
+    }
+  }
+  // fp32: blocks are twice as large and products eight times as long.  The next keys are fetched into the registers of this block's as
+  // soon as its scores are there, the next values into this block's strip as soon as they are in registers.
+  __device__ __forceinline__ void own_one(int kb, int page0, int page) {
+    constexpr int kHop = kWavesWg * kBlockKeys;
+    KFrag kf[2][QF];
+    fetch_own(page0, kb, 0, kf);
+#pragma unroll 1
+    for (bool more = true; more; kb += kHop) {
+      more = kb + kHop < k_end;
+      float4_t sc[NT][2];
+      Probs pf[NT];
+      VFrag vf[DT];
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      scores(kf, sc);
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) fetch_own_k(page, kb + kHop, kf);
+      clean_own(kb, strip_at(0));
+      softmax<true>(sc, kb, pf);
+      read_v(strip_at(0), vf);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) {
+        fetch_own_v(page, kb + kHop, 0);
+        page = page_of(kb + 2 * kHop);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      add_values(vf, pf);
     }
   }
 
