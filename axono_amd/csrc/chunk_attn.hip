@@ -16,8 +16,8 @@
 // address of a stage is inside the pool whatever the lengths are.
 //
 // Few tiles over many keys would leave the device idle: the keys of a tile are cut into pieces so that the launch has
-// about two workgroups per CU (fp32 with D = 64: three) of equal work.  The cut is made on the device from cu_tokens and start (every workgroup
-// derives it with a few wave operations), so a captured launch follows lengths that change.  A piece of a cut tile leaves
+// about two workgroups per CU (fp32 with D = 64: three) of equal work.  The cut is made on the device from cu_tokens and start
+// (every workgroup derives it with a few wave operations), so a captured launch follows lengths that change.  A piece of a cut tile leaves
 // an unnormalised state in the workspace; a second kernel adds the pieces of a tile in a fixed order.  No counters, no
 // state between launches: launches with workspaces of their own may overlap.
 //
@@ -60,10 +60,10 @@ struct Cfg {
   // Column tiles per wavefront, the fewest units of 128 keys of a piece, and the workgroups per CU that the cut aims at.
   // fp32 products take long enough for one column tile, and with half the rows in a tile and pieces of a single unit small
   // batches spread over more workgroups (D = 64, against 2 tiles, 2 units, 2 workgroups): 3 ragged prompts of 200 tokens
-  // 17 us against 29, 16 decoding sequences at 2000 keys 26 against 39, 4096 tokens of one prompt 189 against 220.
-  // A third workgroup fits there only (registers): 189 us against 254 with two; four pieces per CU: 300 tokens at 6000
-  // keys 52 us against 42.  fp16 is slower with pieces of one unit (512 tokens of one prompt 25 us against 23) and gains
-  // nothing from three workgroups (D = 64: 4 x 1000 tokens 64 us against 62; D = 128 has registers for two).
+  // 16 us against 27, 16 decoding sequences at 2000 keys 25 against 31, 4096 tokens of one prompt 167 against 211.  A third
+  // workgroup fits there only (registers): 167 us against 225 with two; four pieces per CU: 300 tokens at 6000 keys 37 us
+  // against 32.  fp16 is slower with pieces of one unit (512 tokens of one prompt 25 us against 23) and gains nothing from
+  // three workgroups (D = 64: 4 x 1000 tokens 64 us against 62; D = 128 has registers for two).
   static constexpr int NT = D == 256 || sizeof(T) == 4 ? 1 : 2;
   static constexpr int MIN = sizeof(T) == 4 ? 1 : 2;
   static constexpr int AIM = D == 64 && sizeof(T) == 4 ? 3 : 2;
@@ -122,7 +122,7 @@ __device__ __forceinline__ int units_per_piece(const ChunkArgs &a, const Seq &fi
 // Pieces of every tile of a sequence.  One that has few rows only streams keys, each its own: shorter pieces spread such
 // streams better over the device (32 sequences of 4000 keys 60 us, 65 us with whole pieces), while tiles of many rows that start
 // together share their keys in the caches.  Pieces that are short anyway stay whole (1 sequence of 32000 keys, pieces of 4 units
-// 39 us, of 2 units 42 us).
+// 35 us, of 2 units 38 us).
 template <typename C>
 __device__ __forceinline__ int pieces_of(const Seq &s, int per) {
   const int p = C::kOwnBlocks && s.rows <= C::FEW && per >= 8 ? (per + 1) / 2 : per;
@@ -889,8 +889,8 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
 
 // Adds the pieces of a cut tile: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  A workgroup takes up to 16 rows of the tile;
 // where these are fewer, or the pieces many, several threads share an element and take every P-th piece each, and their sums
-// are added up in a fixed tree through LDS (one row of 63 pieces: 5.6 us, 8.4 us one after the other): a thread has four pieces on their way at a time, and what bounds this kernel is the
-// chain of such trips (one row of 128 pieces: 8 trips instead of 32).
+// are added up in a fixed tree through LDS (one row of 63 pieces: 5.6 us, 8.4 us one after the other).  A thread has four pieces
+// on their way at a time, and what bounds this kernel is the chain of such trips.
 constexpr int kMergeRows = 16;
 struct Sum {
   float m, l;
