@@ -198,6 +198,8 @@ class Qwen3VLTextDecoder(nn.Module):
             nbytes = self._lib.axhip_decode_layer_tail_workspace_bytes(cfg.hidden_size, cfg.intermediate_size)
             self._tail_ws = Tensor(DataType.INT8, [nbytes], device)
         self._sampling = None   # what a step does to its logits before argmax (start_decode)
+        # ids that prefill() / prefill_chunk() have put into each sequence's cache, None where they are not all known
+        self._prompt = [np.zeros(0, np.int64)] * batch
 
     # ---- pieces ----------------------------------------------------------------------------
     def _w(self, name):
@@ -376,6 +378,7 @@ class Qwen3VLTextDecoder(nn.Module):
                 check(lib.axhip_memcpy_d2d(last_h.data_ptr + (b + j) * H * 2, xn.data_ptr + (j * S + S - 1) * H * 2, H * 2),
                       "copy")
         self._cache.set_lengths(np.full(B, S, np.int32))
+        self._prompt = [row.astype(np.int64) for row in np.asarray(ids)]
         logits = self._linear(last_h, "embed_tokens.weight")
         return logits, L.argmax(logits)
 
@@ -411,6 +414,10 @@ class Qwen3VLTextDecoder(nn.Module):
                                     self._w(p + "post_attention_layernorm.weight"), cfg.rms_norm_eps, DataType.FLOAT16)
             nxt = f"layers.{i + 1}.input_layernorm.weight" if i + 1 < cfg.num_hidden_layers else "norm.weight"
             h, xn = L.add_rms_norm(self._mlp(xn2, p), h, self._w(nxt), cfg.rms_norm_eps, DataType.FLOAT16)
+        for b, have in enumerate(cache.lengths):
+            known = self._prompt[b] if have else new_ids[b][:0]
+            if n[b]:
+                self._prompt[b] = np.concatenate([known, new_ids[b]]) if known is not None and len(known) == have else None
         cache.advance_each(n)
         last = np.cumsum(n)[n > 0] - 1   # rows of the last new tokens
         logits = self._linear(L.embedding(_dev(last, dev), xn), "embed_tokens.weight")
@@ -418,16 +425,21 @@ class Qwen3VLTextDecoder(nn.Module):
 
     # ---- captured decode loop ------------------------------------------------------------------
     def start_decode(self, first_ids: np.ndarray, first_pos: np.ndarray, max_new_tokens: int,
-                     trace: list | None = None, sampling: dict | None = None):
+                     trace: list | None = None, sampling: dict | None = None, prompt_ids=None):
         """Sets the static step inputs (ids [B], positions [3,B]) and captures the step.  The
         attention split plan is sized for the lengths the loop will reach.  `trace`, if given, holds
         after every run of the step (eager, or a replay of the captured one) the residual stream entering
         each layer and the one leaving the last, as decode_forward documents; inside a captured step these
         are the graph's own buffers, refreshed by each replay.  `sampling`, if given, holds what every step does to its
         logits before argmax: keywords of libaxono.logits_process (repetition, presence, frequency, bias_ids, bias, allowed;
-        device tensors, read again by every replay), with the tokens of the loop so far as the history."""
+        device tensors, read again by every replay).  Their history is, of every sequence, the prompt, first_ids and the tokens of
+        the loop so far, also of earlier calls of generate(); presence and frequency count from first_ids on.  `prompt_ids`, if
+        given, holds each sequence's tokens before first_ids (B arrays); by default they are those that prefill() and
+        prefill_chunk() were given, and where the cache holds others a `repetition` penalty needs prompt_ids.  first_ids are the
+        caller's choice: libaxono.logits_process on the prefill's logits applies the same to them."""
         B = self._batch
         self._sampling = None
+        history = self._history_of(first_ids, sampling, prompt_ids) if sampling is not None else None
         self._ids.copy_from_numpy(np.ascontiguousarray(first_ids, dtype=np.int64).reshape(B))
         self._pos.copy_from_numpy(np.ascontiguousarray(first_pos, dtype=np.int64).reshape(3, B))
         bound = min(self._cache.max_len, len(self._cache) + max_new_tokens + 1)
@@ -441,9 +453,19 @@ class Qwen3VLTextDecoder(nn.Module):
         # the tokens of every step are gathered on the device, at the row a device-side counter names
         self._log = Tensor(DataType.INT64, [max(max_new_tokens, 1), B], self._device)
         self._counter = Tensor(DataType.INT64, [1], self._device)
-        self._logged = Tensor(DataType.INT32, [B], self._device)   # rows of the log that hold tokens, for the history
+        self._history = None
         if sampling is not None:
-            self._sampling = {**sampling, "history": self._log, "history_len": self._logged, "by_step": True}
+            # a history [rows, B] of its own: the prompts' ids end at row len - 1, first_ids is the next, the loop's tokens follow
+            # (a step more than generate() may take, and the two of a capture)
+            seen = len(history)
+            rows = np.full((bound - len(self._cache) + 2, B), -1, np.int64)
+            self._history = Tensor.from_numpy_ref(np.concatenate([history, rows])).to(self._device)
+            self._history_len = Tensor(DataType.INT32, [B], self._device)
+            self._history_at = Tensor(DataType.INT64, [1], self._device)
+            self._history_from = (seen, len(self._cache))
+            self._rewind_history()
+            self._sampling = {**sampling, "history": self._history, "history_len": self._history_len, "by_step": True,
+                              "prompt_len": _dev(np.full(B, seen - 1, np.int32), self._device)}
 
         def step():
             if trace is not None:
@@ -452,11 +474,45 @@ class Qwen3VLTextDecoder(nn.Module):
             # the device-side state of the next step, and the token log: one launch
             L.decode_advance(nxt, self._ids, self._pos, self._cache.seq_lens, self._log, self._counter)
             if sampling is not None:
-                L.index_add(self._logged, 1)
+                L.decode_advance(nxt, seq_lens=self._history_len, log=self._history, counter=self._history_at)
             return logits, nxt
 
         self._step_fn = step
         return step
+
+    def _history_of(self, first_ids, sampling, prompt_ids):
+        """[rows, B] ids: every sequence's prompt, aligned at its end (-1 in front: no token's id), and first_ids."""
+        B = self._batch
+        if prompt_ids is not None:
+            prompt_ids = [np.asarray(x, np.int64).reshape(-1) for x in prompt_ids]
+            if len(prompt_ids) != B:
+                raise ValueError(f"start_decode(): prompt_ids of {B} sequences expected, got {len(prompt_ids)}")
+        elif sampling.get("repetition") is not None:
+            lens = self._cache.seq_lens.numpy()
+            prompt_ids = self._prompt
+            for b, known in enumerate(prompt_ids):
+                if known is None or len(known) != lens[b]:
+                    raise ValueError(f"start_decode(): the repetition penalty looks at the {lens[b]} tokens that sequence {b} holds, and "
+                                     "prefill() / prefill_chunk() were not given all of them; pass prompt_ids")
+        else:
+            prompt_ids = [[]] * B                       # the other penalties do not look at it
+        longest = max(len(x) for x in prompt_ids)
+        ids = np.full((longest + 1, B), -1, np.int64)
+        for b, x in enumerate(prompt_ids):
+            ids[longest - len(x):longest, b] = x
+        ids[longest] = np.asarray(first_ids, np.int64).reshape(B)
+        return ids
+
+    def _rewind_history(self):
+        """The history holds what the loop has put into the cache so far (whose length may have been set back)."""
+        if self._history is None:
+            return
+        seen, at = self._history_from
+        done = len(self._cache) - at
+        if done < 0:
+            raise RuntimeError("generate(): the cache holds less than at start_decode(); call start_decode() again")
+        self._history_len.copy_from_numpy(np.full(self._batch, seen + done, np.int32))
+        self._history_at.copy_from_numpy(np.full(1, seen + done, np.int64))
 
     def capture(self):
         """Captures one decode step (after a warm-up run) and rewinds the state both runs advanced."""
@@ -470,7 +526,7 @@ class Qwen3VLTextDecoder(nn.Module):
         self._pos.copy_from_numpy(pos0)
         self._cache.seq_lens.copy_from_numpy(lens0)
         self._counter.copy_from_numpy(np.zeros(1, np.int64))
-        self._logged.fill_zero()
+        self._rewind_history()
         self._graph = g
         self._graph_out = g.outputs
         return g
@@ -489,7 +545,7 @@ class Qwen3VLTextDecoder(nn.Module):
                                f"{self._decode_bound} keys; {have} cached + {max_new_tokens} new exceed that. "
                                f"Call start_decode() (and capture()) again for the new length")
         self._counter.copy_from_numpy(np.zeros(1, np.int64))
-        self._logged.fill_zero()
+        self._rewind_history()
         L.synchronize()
         for _ in range(max_new_tokens):
             if use_graph:

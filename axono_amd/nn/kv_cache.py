@@ -227,6 +227,11 @@ class PagedKVCache(KVCache):
     def pages_in_use(self) -> int:
         return self.n_pages - len(self._free)
 
+    @property
+    def lengths(self) -> np.ndarray:
+        """Every sequence's length, as the host knows it."""
+        return self._lens.copy()
+
     def reserve(self, new_tokens=1) -> None:
         """Makes sure every sequence has pages for its length + new_tokens (an int, or one int per
         sequence).  Raises MemoryError when the pool runs out (nothing is changed then)."""
