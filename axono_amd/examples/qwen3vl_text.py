@@ -140,6 +140,10 @@ def _dev(arr, device):
     return Tensor.from_numpy_ref(np.ascontiguousarray(arr)).to(device)
 
 
+# keywords of libaxono.logits_process that start_decode(sampling=...) takes; the history is the loop's own
+SAMPLING = ("repetition", "presence", "frequency", "bias_ids", "bias", "allowed")
+
+
 class Qwen3VLTextDecoder(nn.Module):
     """paged=True keeps the KV cache in pages of 128 keys (nn.PagedKVCache, `n_pages` per layer pool; default:
     enough for every sequence to reach max_len) instead of one [B, n_kv, max_len, d_head] block per layer; prefill()
@@ -439,6 +443,9 @@ class Qwen3VLTextDecoder(nn.Module):
         caller's choice: libaxono.logits_process on the prefill's logits applies the same to them."""
         B = self._batch
         self._sampling = None
+        unknown = sorted(set(sampling or ()) - set(SAMPLING))
+        if unknown:
+            raise ValueError(f"start_decode(): sampling takes {', '.join(SAMPLING)}, not {', '.join(unknown)}")
         history = self._history_of(first_ids, sampling, prompt_ids) if sampling is not None else None
         self._ids.copy_from_numpy(np.ascontiguousarray(first_ids, dtype=np.int64).reshape(B))
         self._pos.copy_from_numpy(np.ascontiguousarray(first_pos, dtype=np.int64).reshape(3, B))

@@ -157,3 +157,10 @@ def test_a_dense_prefill_is_known_too():
     np.testing.assert_array_equal(other[1], got[0][1])            # the row without a repetition penalty
     for b in (0, 2):
         assert set(np.nonzero(other[b] != got[0][b])[0]) == set(ids[b]) - {nxt.to_numpy()[b]}
+
+
+@pytest.mark.parametrize("key", ["history", "history_len", "prompt_len", "by_step", "out", "temperature"])
+def test_what_the_loop_keeps_itself_or_does_not_know_is_refused(key):
+    gpu, ids, first = started(4)
+    with pytest.raises(ValueError, match=key):
+        gpu.start_decode(first, positions(ids), 4, sampling={**penalties(), key: hip(np.zeros(B, np.int32))})
