@@ -201,7 +201,6 @@ class Qwen3VLTextDecoder(nn.Module):
         if self._fused_tail:
             nbytes = self._lib.axhip_decode_layer_tail_workspace_bytes(cfg.hidden_size, cfg.intermediate_size)
             self._tail_ws = Tensor(DataType.INT8, [nbytes], device)
-        self._sampling = None   # what a step does to its logits before argmax (start_decode)
         # ids that prefill() / prefill_chunk() have put into each sequence's cache, None where they are not all known
         self._prompt = [np.zeros(0, np.int64)] * batch
 
@@ -245,12 +244,14 @@ class Qwen3VLTextDecoder(nn.Module):
         (examples/vlm/qwen3vl/model.py:827-861)."""
         return self.decode_forward(ids, pos)
 
-    def decode_forward(self, ids: Tensor, pos: Tensor, attn_max_len: int | None = None, trace: list | None = None):
+    def decode_forward(self, ids: Tensor, pos: Tensor, attn_max_len: int | None = None, trace: list | None = None,
+                       sampling: dict | None = None):
         """One token per sequence.  ids INT64 [B]; pos INT64 [3,B]; appends to the cache at
         cache.seq_lens and attends over seq_lens + 1 keys.  Returns (logits FLOAT32 [B,V], next ids
         INT64 [B]).  Does not advance the lengths.  `trace`, if given, receives the residual stream
         entering every layer and the one leaving the last (FLOAT32 [B,H] tensors), for layer-wise
-        comparison with a reference evaluation."""
+        comparison with a reference evaluation.  `sampling`, if given, holds keywords of
+        libaxono.logits_process: what is done to the logits before argmax."""
         cfg = self._cfg
         B = self._batch
         cache = self._cache
@@ -300,8 +301,8 @@ class Qwen3VLTextDecoder(nn.Module):
         if trace is not None:
             trace.append(h)
         logits = self._linear(xn, "embed_tokens.weight")  # tied lm_head
-        if self._sampling is not None:
-            logits = L.logits_process(logits, **self._sampling)
+        if sampling is not None:
+            logits = L.logits_process(logits, **sampling)
         return logits, L.argmax(logits)
 
     # ---- prefill -----------------------------------------------------------------------------
@@ -442,7 +443,6 @@ class Qwen3VLTextDecoder(nn.Module):
         prefill_chunk() were given, and where the cache holds others a `repetition` penalty needs prompt_ids.  first_ids are the
         caller's choice: libaxono.logits_process on the prefill's logits applies the same to them."""
         B = self._batch
-        self._sampling = None
         unknown = sorted(set(sampling or ()) - set(SAMPLING))
         if unknown:
             raise ValueError(f"start_decode(): sampling takes {', '.join(SAMPLING)}, not {', '.join(unknown)}")
@@ -471,13 +471,13 @@ class Qwen3VLTextDecoder(nn.Module):
             self._history_at = Tensor(DataType.INT64, [1], self._device)
             self._history_from = (seen, len(self._cache))
             self._rewind_history()
-            self._sampling = {**sampling, "history": self._history, "history_len": self._history_len, "by_step": True,
-                              "prompt_len": _dev(np.full(B, seen - 1, np.int32), self._device)}
+            sampling = {**sampling, "history": self._history, "history_len": self._history_len, "by_step": True,
+                        "prompt_len": _dev(np.full(B, seen - 1, np.int32), self._device)}
 
         def step():
             if trace is not None:
                 del trace[:]
-            logits, nxt = self.decode_forward(self._ids, self._pos, bound, trace=trace)
+            logits, nxt = self.decode_forward(self._ids, self._pos, bound, trace=trace, sampling=sampling)
             # the device-side state of the next step, and the token log: one launch
             L.decode_advance(nxt, self._ids, self._pos, self._cache.seq_lens, self._log, self._counter)
             if sampling is not None:

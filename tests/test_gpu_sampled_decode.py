@@ -164,3 +164,20 @@ def test_what_the_loop_keeps_itself_or_does_not_know_is_refused(key):
     gpu, ids, first = started(4)
     with pytest.raises(ValueError, match=key):
         gpu.start_decode(first, positions(ids), 4, sampling={**penalties(), key: hip(np.zeros(B, np.int32))})
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_a_step_behind_a_sampled_loop_gives_plain_logits(use_graph):
+    """decode_forward and forward take no penalties and masks from a loop that was started before"""
+    def tokens():
+        return hip(np.arange(B, dtype=np.int64)), hip(positions(ids))
+
+    gpu, ids, first = started(6)
+    want = gpu.decode_forward(*tokens())[0].to_numpy().copy()
+    gpu.start_decode(first, positions(ids), 4, sampling=dict(allowed=hip(np.full((B, 32), 5, np.int32)), **penalties()))
+    if use_graph:
+        gpu.capture()
+    assert np.isinf((gpu._graph.replay() and gpu._graph_out if use_graph else gpu._step_fn())[0].to_numpy()).any()
+    gpu.cache.set_lengths([len(i) for i in ids])
+    for step in (gpu.decode_forward, gpu.forward):
+        np.testing.assert_array_equal(step(*tokens())[0].to_numpy(), want)
