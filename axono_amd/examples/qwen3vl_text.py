@@ -431,14 +431,15 @@ class Qwen3VLTextDecoder(nn.Module):
     # ---- captured decode loop ------------------------------------------------------------------
     def start_decode(self, first_ids: np.ndarray, first_pos: np.ndarray, max_new_tokens: int,
                      trace: list | None = None, sampling: dict | None = None, prompt_ids=None):
-        """Sets the static step inputs (ids [B], positions [3,B]) and captures the step.  The
-        attention split plan is sized for the lengths the loop will reach.  `trace`, if given, holds
-        after every run of the step (eager, or a replay of the captured one) the residual stream entering
-        each layer and the one leaving the last, as decode_forward documents; inside a captured step these
-        are the graph's own buffers, refreshed by each replay.  `sampling`, if given, holds what every step does to its
-        logits before argmax: keywords of libaxono.logits_process (repetition, presence, frequency, bias_ids, bias, allowed;
-        device tensors, read again by every replay).  Their history is, of every sequence, the prompt, first_ids and the tokens of
-        the loop so far, also of earlier calls of generate(); presence and frequency count from first_ids on.  `prompt_ids`, if
+        """Sets the static step inputs (ids [B], positions [3,B]) and returns the step, which capture() records and
+        generate() repeats; a graph captured before does not belong to it.  The attention split plan is sized for
+        the lengths the loop will reach.  `trace`, if given, holds after every run of the step (eager, or a replay of
+        the captured one) the residual stream entering each layer and the one leaving the last, as decode_forward
+        documents; inside a captured step these are the graph's own buffers, refreshed by each replay.
+        `sampling`, if given, holds what every step does to its logits before argmax: keywords of
+        libaxono.logits_process (repetition, presence, frequency, bias_ids, bias, allowed; device tensors, read again by
+        every replay).  Their history is, of every sequence, the prompt, first_ids and the tokens of the loop so
+        far, also of earlier calls of generate(); presence and frequency count from first_ids on.  `prompt_ids`, if
         given, holds each sequence's tokens before first_ids (B arrays); by default they are those that prefill() and
         prefill_chunk() were given, and where the cache holds others a `repetition` penalty needs prompt_ids.  first_ids are the
         caller's choice: libaxono.logits_process on the prefill's logits applies the same to them."""
@@ -457,9 +458,10 @@ class Qwen3VLTextDecoder(nn.Module):
         # the captured attention launches attend to at most `bound` keys and append only below it:
         # generate() refuses to run past it (it would silently drop tokens from the cache otherwise)
         self._decode_bound = bound
+        self._graph = self._graph_out = None
         # the tokens of every step are gathered on the device, at the row a device-side counter names
-        self._log = Tensor(DataType.INT64, [max(max_new_tokens, 1), B], self._device)
-        self._counter = Tensor(DataType.INT64, [1], self._device)
+        log = self._log = Tensor(DataType.INT64, [max(max_new_tokens, 1), B], self._device)
+        counter = self._counter = Tensor(DataType.INT64, [1], self._device)
         self._history = None
         if sampling is not None:
             # a history [rows, B] of its own: the prompts' ids end at row len - 1, first_ids is the next, the loop's tokens follow
@@ -468,7 +470,7 @@ class Qwen3VLTextDecoder(nn.Module):
             rows = np.full((bound - len(self._cache) + 2, B), -1, np.int64)
             self._history = Tensor.from_numpy_ref(np.concatenate([history, rows])).to(self._device)
             self._history_len = Tensor(DataType.INT32, [B], self._device)
-            self._history_at = Tensor(DataType.INT64, [1], self._device)
+            history_at = self._history_at = Tensor(DataType.INT64, [1], self._device)
             self._history_from = (seen, len(self._cache))
             self._rewind_history()
             sampling = {**sampling, "history": self._history, "history_len": self._history_len, "by_step": True,
@@ -479,9 +481,9 @@ class Qwen3VLTextDecoder(nn.Module):
                 del trace[:]
             logits, nxt = self.decode_forward(self._ids, self._pos, bound, trace=trace, sampling=sampling)
             # the device-side state of the next step, and the token log: one launch
-            L.decode_advance(nxt, self._ids, self._pos, self._cache.seq_lens, self._log, self._counter)
+            L.decode_advance(nxt, self._ids, self._pos, self._cache.seq_lens, log, counter)
             if sampling is not None:
-                L.decode_advance(nxt, seq_lens=self._history_len, log=self._history, counter=self._history_at)
+                L.decode_advance(nxt, seq_lens=sampling["history_len"], log=sampling["history"], counter=history_at)
             return logits, nxt
 
         self._step_fn = step
@@ -534,6 +536,7 @@ class Qwen3VLTextDecoder(nn.Module):
         self._cache.seq_lens.copy_from_numpy(lens0)
         self._counter.copy_from_numpy(np.zeros(1, np.int64))
         self._rewind_history()
+        g.step = self._step_fn   # a graph that the caller keeps writes to the log and history of its own step
         self._graph = g
         self._graph_out = g.outputs
         return g
@@ -551,6 +554,9 @@ class Qwen3VLTextDecoder(nn.Module):
             raise RuntimeError(f"generate(): the step was set up by start_decode() for sequences of up to "
                                f"{self._decode_bound} keys; {have} cached + {max_new_tokens} new exceed that. "
                                f"Call start_decode() (and capture()) again for the new length")
+        if use_graph and self._graph is None:
+            raise RuntimeError("generate(): start_decode() set up a step that capture() has not recorded yet "
+                               "(or pass use_graph=False)")
         self._counter.copy_from_numpy(np.zeros(1, np.int64))
         self._rewind_history()
         L.synchronize()

@@ -181,3 +181,25 @@ def test_a_step_behind_a_sampled_loop_gives_plain_logits(use_graph):
     gpu.cache.set_lengths([len(i) for i in ids])
     for step in (gpu.decode_forward, gpu.forward):
         np.testing.assert_array_equal(step(*tokens())[0].to_numpy(), want)
+
+
+def test_a_new_loop_needs_a_capture_of_its_own():
+    """the graph of the loop before applies that loop's penalties and writes to its log"""
+    gpu, ids, first = started(7)
+    gpu.start_decode(first, positions(ids), 4)
+    with pytest.raises(RuntimeError, match="capture"):
+        gpu.generate(4)
+    old = gpu.capture()
+    gpu.start_decode(first, positions(ids), 4, sampling=dict(allowed=hip(np.full((B, 32), 5, np.int32))))
+    with pytest.raises(RuntimeError, match="capture"):
+        gpu.generate(4)
+    assert gpu.generate(0, use_graph=False).shape == (0, B)
+    gpu.capture()
+    log = gpu._log.to_numpy().copy()
+    old.replay()                                    # into its own log
+    np.testing.assert_array_equal(gpu._log.to_numpy(), log)
+    gpu._ids.copy_from_numpy(first.astype(np.int64))
+    gpu._pos.copy_from_numpy(positions(ids))
+    gpu.cache.set_lengths([len(i) for i in ids])
+    toks = gpu.generate(4)
+    assert np.all((5 >> (toks % 32)) & 1)
