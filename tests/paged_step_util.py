@@ -138,13 +138,14 @@ def append(qkv, hq, hk, w, eps, norm, pos, axes, freq, scale, interleaved, rd, s
 
 
 # ---- attention -----------------------------------------------------------------------------------------------------------
-def chunk_want(q, k_pool, v_pool, table, n, start, max_len):
+def chunk_want(q, k_pool, v_pool, table, n, start, max_len, lost=2.0 ** -25):
     """softmax over the keys that a token sees, in 64 bits; and the bound of a right result's error:
     - a score is a sum of D products in fp32: D 2^-24 sum |q k| scale; the argument of the exponential, of size A, rounds twice
       and the exponential itself is good to 2^-22: every probability is off by d = that sum, relative;
-    - fp16: a probability rounds to fp16, 2^-11 relative, or 2^-25 absolute where it is tiny (the largest is at least 1);
+    - fp16: a probability rounds to fp16, 2^-11 relative, or `lost` absolute where it is tiny (the largest is at least 1; 2^-25 where
+      it is held as it is, 2^-35 where the largest is held at 2^10 at least);
     - numerator and denominator are sums of n terms in fp32: n 2^-24 each;
-    - the result rounds once.  With W = sum p |v| / sum p the error is at most W (2 d + 2 u + 2 n 2^-24) + n 2^-25 max |v|
+    - the result rounds once.  With W = sum p |v| / sum p the error is at most W (2 d + 2 u + 2 n 2^-24) + n lost max |v|
       (fp16 only; the maximum over the keys of that element) + |out| u."""
     T, hq, d = q.shape
     hk, g = k_pool.shape[1], hq // k_pool.shape[1]
@@ -176,7 +177,7 @@ def chunk_want(q, k_pool, v_pool, table, n, start, max_len):
                         2 * np.abs(s - top).max() * 2.0 ** -24 * 1.5 + np.abs(top).max() * 2.0 ** -23 + 2.0 ** -22
                     e = W * (2 * delta + 2 * m * 2.0 ** -24 + (2 * U[t_] if half else 0)) + np.abs(o) * U[t_] + TINY[t_]
                     if half:
-                        e = e + m * 2.0 ** -25 * np.abs(V[:m]).max(0)
+                        e = e + m * lost * np.abs(V[:m]).max(0)
                 out[cu[b] + i, h * g:(h + 1) * g] = o
                 tol[cu[b] + i, h * g:(h + 1) * g] = e
     return out, tol
@@ -195,6 +196,50 @@ def chunk(q, k_pool, v_pool, table, cu, start, max_q, max_len, fill=9.0, tokens=
                                             table.shape[1], k_pool.shape[0], None), "chunk_attention_paged")
     synchronize()
     return out.download(q.dtype, q.shape)
+
+
+# Inputs whose results are whole numbers over whole numbers, so that one key too few, too many, taken twice or taken from another
+# place shows: K holds 0 and -240, V 1 and -1, a query 8 in one place and 0 elsewhere.  The keys that have 0 in that place weigh 1, the
+# others 2^-170 and less, which is nothing in either type: a row's result is the sum of its keys' values over their number.
+def picking(n, start, hq, hk, d, dtype, seed=0):
+    rng = np.random.default_rng(seed)
+    table, n_pages = pages_for(n, start, rng)
+    T = sum(n)
+    q = np.zeros((T, hq, d), dtype)
+    row = np.arange(T * hq)
+    q.reshape(-1, d)[row, (7 * row + row // d) % d] = 8
+    k = (-240 * rng.integers(0, 2, (n_pages, hk, 128, d))).astype(dtype)
+    v = (2 * rng.integers(0, 2, (n_pages, hk, 128, d)) - 1).astype(dtype)
+    return q, k, v, table
+
+
+def picking_want(q, k_pool, v_pool, table, n, start, keys_of=None):
+    """(sums [T, hq, d], numbers of keys [T, hq]); keys_of(b, m): the keys that a row with m visible ones takes (an oracle with a
+    mistake in it), all m by default"""
+    T, hq, d = q.shape
+    hk, g = k_pool.shape[1], hq // k_pool.shape[1]
+    sums, numbers = np.zeros((T, hq, d)), np.zeros((T, hq))
+    cu = cu_of(n)
+    for b in range(len(n)):
+        pages = table[b, :(int(start[b]) + int(n[b]) + PAGE - 1) // PAGE]
+        for h in range(hk):
+            K, V = (p[pages, h].reshape(-1, d).astype(np.float32) for p in (k_pool, v_pool))
+            for i in range(n[b]):
+                m = int(start[b]) + i + 1
+                at = np.arange(m) if keys_of is None else keys_of(b, m)
+                x = q[cu[b] + i, h * g:(h + 1) * g].argmax(-1)
+                taken = (K[at][:, x] == 0).T
+                taken[~taken.any(-1)] = True            # they all weigh the same then
+                sums[cu[b] + i, h * g:(h + 1) * g] = taken.astype(np.float32) @ V[at]
+                numbers[cu[b] + i, h * g:(h + 1) * g] = taken.sum(-1)
+    return sums, numbers
+
+
+def picking_error(got, sums, numbers):
+    """largest distance of result * number from the sum: under 1 / 4 for a right result in fp16 too, whose rounding of sums up to
+    500 is half a step, 500 * 2^-11"""
+    assert np.abs(sums).max() <= 500
+    return np.abs(got.astype(np.float64) * numbers[..., None] - sums).max()
 
 
 # ---- logits ----------------------------------------------------------------------------------------------------------------
