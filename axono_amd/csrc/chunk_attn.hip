@@ -428,6 +428,9 @@ struct Wave {
   // 2^-24 of the largest weight of a row its others lose bits, below 2^-35 they are lost.  (Against the maximum itself those
   // under 2^-25 would be, and 65536 such keys hold 2^-9 of the sum.)
   static constexpr float kBelow = kHalf ? 10.f : 0.f, kTop = kHalf ? 32768.f : 256.f;
+  // Large scores: the level is a product rounded to fp32, taken a step or two low so that the largest score never lies under what it
+  // was meant to be over.  Where a step is more than kTop leaves room for (levels past 2^23) p ends at kTop: scores within
+  // 2^-22 of the largest then weigh the same, which is what the rounding of their own sums leaves of them.
   // MASK: some key of the block at kb is behind some row's position.
   template <bool MASK>
   __device__ __forceinline__ void softmax(const float4_t (&sc)[NT][2], int kb, Probs (&pf)[NT]) {
@@ -444,7 +447,8 @@ struct Wave {
         float mx = score<MASK>(sc, kb, t, 0);
 #pragma unroll
         for (int j = 1; j < 8; ++j) mx = fmaxf(mx, score<MASK>(sc, kb, t, j));
-        const float mnew = fmaxf(m[t], max_xor32(max_xor16(mx)) * a.scale_log2e - kBelow);
+        const float level = __builtin_fmaf(max_xor32(max_xor16(mx)), a.scale_log2e, -kBelow);
+        const float mnew = fmaxf(m[t], level * (level > 0.f ? 1.f - 0x1p-23f : 1.f + 0x1p-23f));
         const float corr = __builtin_amdgcn_exp2f(m[t] - mnew);
         m[t] = mnew;
         lsum[t] *= corr;
@@ -452,6 +456,10 @@ struct Wave {
         for (int dt = 0; dt < DT; ++dt) o[t][dt] *= corr;
       }
       exps<MASK>(sc, kb, p);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[t][j] = p[t][j] > kTop ? kTop : p[t][j];  // (a NaN stays one)
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
