@@ -40,7 +40,7 @@ constexpr int kWavesWg = 4;
 constexpr int kPageKeys = 128, kPageShift = 7;
 constexpr int kBlockKeys = 32;      // keys of one softmax step
 constexpr int64_t kMostWorkgroups = (1 << 24) - 1;  // a launch has less than 2^32 threads
-constexpr float kMasked = -1.0e30f;
+constexpr float kMasked = -3.40282347e38f;  // below every finite score
 typedef float float8_t __attribute__((ext_vector_type(8)));
 
 struct ChunkArgs {

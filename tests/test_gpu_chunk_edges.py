@@ -71,3 +71,11 @@ FAR = [([1, 3], [0, 700]), ([6], [9000]), ([150], [0]), ([140, 2], [700, 3]), ([
 def test_scores_whose_multiples_of_the_scale_round_by_more_than_one(dtype, top, heads, down, batch):
     """up to 256 * 57344^2 / 16 = 5e10 in fp16: a step of fp32 is 4096 there"""
     largest_wins(*FAR[batch], *heads, dtype, top, down)
+
+
+@pytest.mark.parametrize("top", [57344.0 * 2.0 ** 36, 57344.0 * 2.0 ** 41])
+@pytest.mark.parametrize("heads", [(4, 2, 64), (2, 1, 128), (2, 2, 256)])
+@pytest.mark.parametrize("batch", range(len(FAR)))
+def test_finite_scores_of_any_size_are_no_masked_ones(top, heads, batch):
+    """fp32 scores of -1e32 and -1e35 and a sixteenth of them, nothing above"""
+    largest_wins(*FAR[batch], *heads, np.float32, top, True)
