@@ -80,7 +80,8 @@ struct Cfg {
   // wavefronts with keys of their own in a tile of few rows
   static constexpr int kDealt = kOwnBlocks ? kWavesWg : (KS / kBlockKeys < kWavesWg ? KS / kBlockKeys : kWavesWg);
   static constexpr int kStateBytes = kDealt * FEW * (STATE + 2) * 4;
-  static constexpr int kLdsBytes = (kStageBytes > kStateBytes ? kStageBytes : kStateBytes) + 16;
+  static constexpr int kTail = kStageBytes > kStateBytes ? kStageBytes : kStateBytes;  // where the flags are
+  static constexpr int kLdsBytes = kTail + 16 + TR * 4;
 };
 
 // ---- the cut -------------------------------------------------------------------------------------------------------
@@ -257,7 +258,9 @@ struct Wave {
   typedef const int32_t __attribute__((address_space(4))) *scalar_ptr;
   scalar_ptr table;
   lds_byte *smem;
-  int *flag;                         // some unit of V was cleaned
+  // flags[0]: some unit of V was cleaned; flags[1]: some result is a NaN that its row's sum does not explain; row_nan[r]: row r's
+  // sum is a NaN
+  int *flags, *row_nan;
   KFrag qf[NT][QF];
   float4_t o[NT][DT], lsum[NT];
   float m[NT];
@@ -270,7 +273,8 @@ struct Wave {
     c = lane & 15;
     g = lane >> 4;
     smem = (lds_byte *)chunk_smem;
-    flag = reinterpret_cast<int *>(chunk_smem + C::kLdsBytes - 16);
+    flags = reinterpret_cast<int *>(chunk_smem + C::kTail);
+    row_nan = flags + 4;
     row0 = pc.tile * C::TR;
     n_rows = min(pc.rows - row0, C::TR);
     // rows past the tile repeat its last one and are not stored
@@ -331,7 +335,8 @@ struct Wave {
     }
   }
 
-  // Zero probability times infinity or NaN is NaN, so V must not hold any where some row of the tile does not see its key.
+  // Zero probability times infinity or NaN is NaN.  Where every row of the tile sees the key finish() sets that right; V must not
+  // hold any where some row does not.
   // clean(): a 16-byte unit of V of key `key` in LDS becomes zeros behind the piece's last key, and loses its infinities and
   // NaN (true: it had some); finish() gives them at the end to the rows that see them.  Keys from mixed_from on, a multiple
   // of KS, are cleaned: every key that some row does not see is among them, and every key behind the last.
@@ -532,7 +537,7 @@ struct Wave {
 #pragma unroll 1
       for (int p = 0; p < C::VEC; ++p)
         bad |= clean(smem + kTensor + buf * (KS * kRow) + (p * kThreads + tid) * 16, key0 + p * kStep + tid / UPR);
-      if (bad) *flag = 1;
+      if (bad) flags[0] = 1;
     }
   }
   static __device__ __forceinline__ void products(bool on) {
@@ -550,7 +555,7 @@ struct Wave {
     load_q();
     asm volatile("" ::: "memory");  // the queries' loads are issued before the stages'
     load_stage(page0, k0, 0);
-    lds_barrier();  // the flag is cleared
+    lds_barrier();  // the flags are cleared
     if (n_stages > 1) {
       load_stage(page1, k0 + KS, 1);
       stage_arrived<true>(k0, 0);
@@ -679,7 +684,7 @@ struct Wave {
       bool bad = false;
 #pragma unroll 1
       for (int p = 0; p < kLoads; ++p) bad |= clean(smem + strip + p * 1024 + lane * 16, kb + (p * 64 + lane) / UPR);
-      if (bad) *flag = 1;
+      if (bad) flags[0] = 1;
     }
   }
   __device__ __forceinline__ void use_own(int kb, int buf, const KFrag (&kf)[2][QF]) {
@@ -696,7 +701,7 @@ struct Wave {
   }
   __device__ __forceinline__ void own_blocks() {
     constexpr int kHop = kWavesWg * kBlockKeys;
-    lds_barrier();  // the flag is cleared
+    lds_barrier();  // the flags are cleared
     int kb = k0 + wave * kBlockKeys;
     if (kb >= k_end) return;
     const int page0 = page_of(kb);
@@ -776,6 +781,12 @@ struct Wave {
     for (int t = 0; t < NT; ++t) {
       const int r = wrow + t * 16 + c;
       if (r >= n_rows) continue;
+      const bool nan = lsum[t][0] != lsum[t][0];
+      float all = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) all += (o[t][dt][0] + o[t][dt][1]) + (o[t][dt][2] + o[t][dt][3]);
+      if (all != all && !nan) flags[1] = 1;  // (also infinities of both signs, which finish() leaves as they are)
+      if (g == 0) row_nan[r] = nan;
       if (part >= 0) {
         float *po = a.part_o + (part + r) * D;
 #pragma unroll
@@ -829,6 +840,8 @@ struct Wave {
         l = __builtin_fmaf(f, sml[2 * (w * C::FEW + r) + 1], l);
         acc = add_weighted(acc, f, so[(w * C::FEW + r) * C::STATE + d]);
       }
+      if (acc != acc && l == l) flags[1] = 1;
+      if (d == 0) row_nan[r] = l != l;
       if (part >= 0) {
         a.part_o[(part + r) * D + d] = acc;
         if (d == 0) {
@@ -840,23 +853,51 @@ struct Wave {
       }
     }
   }
-  // Infinities and NaN of V that were cleaned away, added to element d of every row that sees their key (a positive weight does
-  // not change them): rare, so through memory and without a thought for speed.
-  __device__ __forceinline__ void finish(bool had, int64_t part) {
-    if (!had) return;
+  // What the values that every row sees hold in element d: 1 infinities, 2 negative ones, 4 NaN.
+  __device__ __forceinline__ void find_kinds(int *kinds) const {
+    for (int d = tid; d < D; d += kThreads) kinds[d] = 0;
+    __syncthreads();
+    const int64_t n = static_cast<int64_t>(max(min(mixed_from, k_end) - k0, 0)) * UPR;
+#pragma unroll 1
+    for (int64_t x = tid; x < n; x += kThreads) {
+      const int key = k0 + static_cast<int>(x / UPR), d = static_cast<int>(x % UPR) * C::E;
+      const T *at = vbase + key_at(table[key >> kPageShift], key) + d;
+      if (!unit_bad<T>(*reinterpret_cast<const u32x4_t *>(at))) continue;
+#pragma unroll 1
+      for (int e = 0; e < C::E; ++e) {
+        const float v = ldf(at + e);
+        if (!(fabsf(v) < __builtin_inff())) atomicOr(kinds + d + e, v != v ? 4 : (v > 0.f ? 1 : 2));
+      }
+    }
+    __syncthreads();
+  }
+  // Infinities and NaN of V as every row that sees their key has them, whatever it weighs: those that were cleaned away are added, and
+  // a NaN that comes from a weight that rounds to 0 becomes the infinity.  Rare, so through memory and without a thought for speed.
+  // (Looking for such a NaN at the end of every piece: 16 x 4096 tokens of 16 heads of 128 in fp16 1142 -> 1150 us.)
+  __device__ __forceinline__ void finish(int64_t part) {
+    lds_barrier();
+    const bool cleaned = flags[0] != 0, odd = flags[1] != 0;
+    if (!cleaned && !odd) return;
     __threadfence_block();
     __syncthreads();
+    int *kinds = reinterpret_cast<int *>(chunk_smem);
+    if (odd) find_kinds(kinds);
     for (int x = tid; x < n_rows * D; x += kThreads) {
       const int r = x / D, d = x % D, last = position(r);
       float sum = 0.f;
-      for (int key = max(k0, mixed_from); key < k_end && key <= last; ++key) {
-        const float v = ldf(vbase + key_at(table[key >> kPageShift], key) + d);
-        if (!(fabsf(v) < __builtin_inff())) sum += v;
+      if (cleaned) {
+        for (int key = max(k0, mixed_from); key < k_end && key <= last; ++key) {
+          const float v = ldf(vbase + key_at(table[key >> kPageShift], key) + d);
+          if (!(fabsf(v) < __builtin_inff())) sum += v;
+        }
       }
-      if (sum == 0.f) continue;
+      const int kind = odd && !row_nan[r] ? kinds[d] : 0;
+      if (sum == 0.f && kind == 0) continue;
       T *out = static_cast<T *>(a.out) + row_at(r) + d;
-      if (part >= 0) a.part_o[(part + r) * D + d] += sum;
-      else stf(out, ldf(out) + sum);
+      float v = part >= 0 ? a.part_o[(part + r) * D + d] : ldf(out);
+      if (v != v && (kind == 1 || kind == 2)) v = kind == 1 ? __builtin_inff() : -__builtin_inff();
+      if (part >= 0) a.part_o[(part + r) * D + d] = v + sum;
+      else stf(out, v + sum);
     }
   }
 };
@@ -875,23 +916,20 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
     if (slot < 0 || slot >= a.slots || n_rows > a.slot_rows) return;  // (only where cu falls and rises: the cut is bounded by both)
     part = slot * a.slot_rows;
   }
-  int *flag = reinterpret_cast<int *>(chunk_smem + C::kLdsBytes - 16);
-  if (threadIdx.x == 0) *flag = 0;
+  if (threadIdx.x < 2) reinterpret_cast<int *>(chunk_smem + C::kTail)[threadIdx.x] = 0;
   if (n_rows <= C::FEW) {
     W w(a, pc, hk, true);
     if constexpr (C::kOwnBlocks) w.own_blocks();
     else w.shared_stages(true);
     __syncthreads();
-    const bool had = *flag != 0;
     w.store_sum(part);
-    w.finish(had, part);
+    w.finish(part);
   } else {
     W w(a, pc, hk, false);
     w.shared_stages(false);
     __syncthreads();
-    const bool had = *flag != 0;
     w.store_rows(part);
-    w.finish(had, part);
+    w.finish(part);
   }
 }
 

@@ -453,7 +453,8 @@ AXHIP_API int axhip_rotary_append_paged(const void *q, int64_t q_stride, const v
  *   workspace: axhip_chunk_attention_paged_workspace_bytes(...) bytes, 16-byte aligned, contents free; launches
  *   that may overlap in time need one each (captured graphs that replay side by side too)
  * Page numbers outside [0, n_pages) are clamped into the pool: wrong values, never an access outside it.  Infinities and
- * NaN in keys and values reach only rows that see them.  Same bits from run to run.
+ * NaN in keys and values reach only rows that see them; a row that sees one among the values has it, whatever it weighs.  Keys with
+ * a score of -infinity weigh nothing; a row that has no others: zeros.  Same bits from run to run.
  * Counterpart of ops::cuda::ScaledDotProductAttention with is_causal (src/ops/cuda/sequence.cu:105-163,451-472), which
  * takes one sequence of dense tensors. */
 AXHIP_API size_t axhip_chunk_attention_paged_workspace_bytes(int dtype, int tokens, int B, int Hq, int Hkv, int D, int max_q,

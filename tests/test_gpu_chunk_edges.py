@@ -79,3 +79,69 @@ def test_scores_whose_multiples_of_the_scale_round_by_more_than_one(dtype, top, 
 def test_finite_scores_of_any_size_are_no_masked_ones(top, heads, batch):
     """fp32 scores of -1e32 and -1e35 and a sixteenth of them, nothing above"""
     largest_wins(*FAR[batch], *heads, np.float32, top, True)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("heads", [(4, 2, 64), (2, 1, 128), (2, 2, 256)])
+@pytest.mark.parametrize("batch", [([6], [1000]), ([6], [9000]), ([150], [700]), ([150, 3], [9000, 300]), ([300], [0]), ([1], [40])])
+def test_infinities_reach_every_row_that_sees_them_whatever_they_weigh(dtype, heads, batch):
+    """Values with infinities and NaN at keys of which half the rows hold the largest score so far and the others e^-300 of it, in
+    places that all rows of a tile see and in places that some do not; early keys, whose weight is large until later ones come,
+    among them.  A weight is never 0: the sum with such a value is what it is for any weight."""
+    (n, start), (hq, hk, d) = batch, heads
+    rng = np.random.default_rng(d)
+    table, n_pages = ps.pages_for(n, start, rng)
+    q = (0.5 * rng.standard_normal((sum(n), hq, d))).astype(dtype)
+    q[..., 0] = 16 * (2 * rng.integers(0, 2, q.shape[:2]) - 1)     # the sign says which of the marked keys are far below
+    k = rng.standard_normal((n_pages, hk, 128, d)).astype(dtype)
+    k[..., 0] = 0
+    v = rng.standard_normal(k.shape).astype(dtype)
+    marked = {}                                                    # key: (dim, value)
+    for b in range(len(n)):
+        last = start[b] + n[b] - 1
+        for i, key in enumerate(sorted({0, 3, 31, min(64, last), last // 3, last // 2, max(last - 70, 0), max(last - 2, 0), last})):
+            if key > last:
+                continue
+            k[table[b, key // 128], :, key % 128, 0] = (1 if i % 2 else -1) * 300 / 16 * np.sqrt(d)
+            v[table[b, key // 128], :, key % 128, 3 + i] = [np.inf, -np.inf, np.nan][i % 3]
+            if i:
+                v[table[b, key // 128], :, key % 128, 20] = np.inf if i != 4 else -np.inf
+    k[..., 1] = q[..., 1] = 0
+    got = ps.chunk(q, k, v, table, ps.cu_of(n), start, max(n), max(s + m for s, m in zip(start, n)))
+    want, tol = ps.chunk_want(q, k, v, table, n, start, max(s + m for s, m in zip(start, n)))
+    assert not np.isfinite(want).all() and np.isfinite(want).any()
+    fine = np.isfinite(want)
+    ps.assert_within(got, want, np.where(fine, tol, 0))
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("n", [6, 150])
+def test_a_row_whose_scores_are_no_numbers_stays_one_without(dtype, n):
+    """a NaN or an infinite score makes the whole row NaN, also where a value that it sees is infinite"""
+    q, k, v, table = ps.picking([n], [900], 4, 2, 64, dtype)
+    v[table[0, 0], :, 5, 7] = np.inf
+    k[table[0, 0], :, 6, :] = np.nan
+    assert np.isnan(ps.chunk(q, k, v, table, ps.cu_of([n]), [900], n, 900 + n)).all()
+    k[table[0, 0], :, 6, :] = np.inf            # queries hold zeros, too: 0 * inf
+    assert np.isnan(ps.chunk(q, k, v, table, ps.cu_of([n]), [900], n, 900 + n)).all()
+    k[table[0, 0], :, 6, :] = 0
+    q[...] = 1
+    k[table[0, 0], 0, 6, 9] = np.inf            # a score of +inf in the first kv head
+    got = ps.chunk(q, k, v, table, ps.cu_of([n]), [900], n, 900 + n)
+    assert np.isnan(got[:, :2]).all() and np.all(got[:, 2:, 7] == np.inf) and np.isfinite(np.delete(got[:, 2:], 7, -1)).all()
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("n,start", [(6, 300), (150, 700), (6, 9000)])
+def test_scores_of_minus_infinity(dtype, n, start):
+    """such a key weighs nothing; a row that has no other comes out as zeros"""
+    q, k, v, table = ps.picking([n], [start], 4, 2, 64, dtype)
+    q[...] = 1
+    k[...] = 0
+    k[table[0], 0, :, 5] = -np.inf              # the first kv head: every key
+    k[table[0, 1], 1, 3:90, 5] = -np.inf        # the second: some
+    got = ps.chunk(q, k, v, table, ps.cu_of([n]), [start], n, start + n)
+    assert np.all(got[:, :2] == 0)
+    gone = np.arange(131, 218)
+    sums, numbers = ps.picking_want(q[:, 2:], k[:, 1:], v[:, 1:], table, [n], [start], lambda b, m: np.setdiff1d(np.arange(m), gone))
+    assert ps.picking_error(got[:, 2:], sums, numbers) <= 0.25
