@@ -5,8 +5,9 @@
 // a = pos * f_i:  y0 = s (x0 cos a - x1 sin a), y1 = s (x1 cos a + x0 sin a); elements behind rotary_dim are copied.
 //
 // The angle of a far position needs more than 32 bits: pos * f in fp32 is off by pos * 2^-24 radians (0.03 at 2^19).
-// It is formed in fp64 as a number of turns, whole turns are dropped, and the rest - below half a turn, exact to
-// 2^-25 - goes to sincosf.  One angle per (token, pair), shared by the heads: a few fp64 instructions per token and lane.
+// It is formed in fp64 as a number of turns, whole turns are dropped, and what is left - below half a turn - goes to sincosf in
+// fp32; the r that this cuts off (up to 2^-23) comes back as cos a - r sin a, sin a + r cos a.  One angle per (token, pair), shared by
+// the heads: a few fp64 instructions per token and lane.
 //
 // Both kernels are bound by HBM (every element is read once and written once: 33001 rows of 24 heads of 128 in fp32 136 us =
 // 6.0 TB/s, 65536 such rows with norm into fp16 pages 285 us = 5.7 TB/s, a plain copy 5.1 TB/s), by the launch when rows are
@@ -189,11 +190,12 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
       p = a.pos[axis * a.rows + t];
     }
     const double turns = static_cast<double>(p) * static_cast<double>(a.inv_freq[i]) * 0.15915494309189533577;  // 1 / 2 pi
-    const float ang = static_cast<float>((turns - rint(turns)) * 6.283185307179586477);
+    const double angle = (turns - rint(turns)) * 6.283185307179586477;
+    const float ang = static_cast<float>(angle), rest = static_cast<float>(angle - static_cast<double>(ang));
     float sn, cs;
     sincosf(ang, &sn, &cs);
-    s_cos[wave][i] = cs * a.scale;
-    s_sin[wave][i] = sn * a.scale;
+    s_cos[wave][i] = __builtin_fmaf(-rest, sn, cs) * a.scale;
+    s_sin[wave][i] = __builtin_fmaf(rest, cs, sn) * a.scale;
   }
   // LDS accesses of one wavefront complete in order; the compiler must keep them in order too
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

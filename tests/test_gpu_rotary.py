@@ -184,3 +184,23 @@ def test_append_same_bits_as_rotary_and_copy():
     np.testing.assert_array_equal(q, wq)
     np.testing.assert_array_equal(kp[table_[0, at // 128], :, at % 128], wk)
     np.testing.assert_array_equal(vp[table_[0, at // 128], :, at % 128], qkv[:, 8:])
+
+
+@pytest.mark.parametrize("append", [False, True])
+def test_cosine_and_sine_are_those_of_the_angle_in_64_bits(append):
+    """(1, 0) turns into cosine and sine: half a step of the value from each of two roundings, a step of sincosf; below 1 a step is
+    2^-24 at most.  An angle near pi cut to 32 bits is off by 2^-23 alone."""
+    rng = np.random.default_rng(12)
+    d, T = 128, 2000
+    pos, f = rng.integers(0, 1 << 20, T), table(d, 1e4)
+    x = np.zeros((T, 2, d), np.float32)
+    x[..., :d // 2] = 1
+    if append:
+        qkv = np.concatenate([x, x[:, :2]], axis=1)
+        table_, n_pages = ps.pages_for([T], [0], rng)
+        pools = [np.zeros((n_pages, 1, 128, d), np.float32) for _ in range(2)]
+        got, _, _ = ps.append(qkv, 2, 1, [None, None], 1e-6, False, pos[None], 1, f, 1.0, False, d, (0, 0), ps.cu_of([T]), [0], table_, *pools)
+    else:
+        got, _ = ps.rotary_qk(x, None, pos, f, 1.0, False, d)
+    want, _ = ps.turned(x, pos, f, d, False, 1.0)
+    assert np.abs(got.astype(np.float64) - want).max() <= 2 * 2.0 ** -24
