@@ -145,3 +145,58 @@ def test_scores_of_minus_infinity(dtype, n, start):
     gone = np.arange(131, 218)
     sums, numbers = ps.picking_want(q[:, 2:], k[:, 1:], v[:, 1:], table, [n], [start], lambda b, m: np.setdiff1d(np.arange(m), gone))
     assert ps.picking_error(got[:, 2:], sums, numbers) <= 0.25
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("heads", [(9, 3, 64), (7, 1, 128), (2, 2, 256)])
+def test_many_sequences_over_long_caches(dtype, heads):
+    """more sequences than lanes whose tiles are cut: the search for a piece, and for the tile to merge, over several loads"""
+    rng = np.random.default_rng(3)
+    n, start = rng.integers(0, 4, 150), rng.integers(0, 3000, 150)
+    n[77], n[140], start[3], start[149], n[149] = 90, 200, 15000, 9000, 2
+    q, k, v, table = ps.picking(list(n), list(start), *heads, dtype)
+    got = ps.chunk(q, k, v, table, ps.cu_of(n), start, 200, int((n + start).max()))
+    assert ps.picking_error(got, *ps.picking_want(q, k, v, table, n, start)) <= 0.25
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("max_len", [4097, 4224, 5000])
+def test_max_len_of_a_cut_tile(dtype, max_len):
+    """tokens behind max_len see the keys before it"""
+    n, start = [300, 2], [4000, 8000]
+    q, k, v, table = ps.picking(n, start, 4, 2, 128, dtype)
+    got = ps.chunk(q, k, v, table, ps.cu_of(n), start, 300, max_len)
+    sums, numbers = ps.picking_want(q, k, v, table, n, start, lambda b, m: np.arange(min(m, max_len)))
+    assert ps.picking_error(got, sums, numbers) <= 0.25
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_captured_calls_follow_what_is_cut(dtype):
+    """one graph, replayed over lengths whose tiles are cut and over others whose are not, of few rows and of many"""
+    from axono_amd import HIPGraph, Tensor, libaxono as L
+
+    def hip(a):
+        return Tensor.from_numpy_ref(np.ascontiguousarray(a)).to("hip:0")
+
+    T, B, hq, hk, d, longest = 120, 3, 4, 2, 64, 9200
+    lots = [([1, 1, 1], [9000, 20, 300]), ([110, 4, 1], [0, 9100, 64]), ([0, 120, 0], [5, 0, 7]), ([2, 90, 3], [700, 9000, 0]), ([1, 0, 1], [0, 0, 127])]
+    at = [hip(np.zeros(s, t)) for s, t in (((T, hq, d), dtype), ((230, hk, 128, d), dtype), ((230, hk, 128, d), dtype), ((B, 73), np.int32),
+                                           ((B + 1,), np.int32), ((B,), np.int32))]
+    g, out = HIPGraph(), []
+    g.capture(lambda: out.append(L.chunk_attention_paged(*at, T, longest)))
+    for seed in (0, 1):
+        for n, start in lots:
+            q, k, v, table = ps.picking(n, start, hq, hk, d, dtype, seed)
+            wide = np.full((B, 73), -1, np.int32)
+            wide[:, :table.shape[1]] = table
+            pool = np.full((2, 230, hk, 128, d), np.nan, dtype)     # (NaN where no sequence has a page)
+            pool[0, :len(k)], pool[1, :len(v)] = k, v
+            rows = np.zeros((T, hq, d), dtype)
+            rows[:len(q)] = q
+            for a, x in zip(at, (rows, pool[0], pool[1], wide, ps.cu_of(n), np.array(start, np.int32))):
+                a.copy_from_numpy(x)
+            g.replay()
+            got = out[-1].numpy()[:len(q)]
+            assert ps.picking_error(got, *ps.picking_want(q, k, v, table, n, start)) <= 0.25, (n, start)
+            eager = L.chunk_attention_paged(*at, T, longest)
+            np.testing.assert_array_equal(eager.numpy()[:len(q)].view(np.uint8), got.view(np.uint8))
