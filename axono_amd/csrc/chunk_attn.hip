@@ -7,7 +7,7 @@
 // wavefronts takes a tile of up to 64 NT rows of one (sequence, kv head) and a piece of the keys they see; a wavefront
 // takes NT column tiles of 16 rows.  In a tile with few rows (at most 16 NT: decoding sequences, drafts, the last rows of
 // a chunk) all wavefronts take the same rows and deal the keys among themselves in blocks of 32; their states are added up at
-// the end.
+// the end.  (D = 256: a stage is one block, so one wavefront multiplies there and the others only load.)
 //
 // Everything is computed transposed, so that no operand changes its layout in registers (see the products below):
 //   S^T = K . Q^T  (16 keys x 16 rows), O^T += V^T . P^T  (16 d x 16 rows); a lane owns the row lane % 16 in both.
@@ -21,10 +21,11 @@
 // an unnormalised state in the workspace; a second kernel adds the pieces of a tile in a fixed order.  No counters, no
 // state between launches: launches with workspaces of their own may overlap.
 //
-// What bounds it, fp16 D = 128: from about 32 rows of a kv head on the matrix cores beside the exponentials (16 x 4096 tokens 1150 us =
-// 955 TFLOP/s, 2048 tokens at 129024 keys 1985 us = 1095 TFLOP/s, where a large library product reaches 1144); below that the
-// stream of keys (4 tokens each of 32 sequences, 573 MB: 6.0 TB/s, with the merge 111 us) and, where there are few keys too, the
-// plan, the merge and the two launches (about 5 us).
+// What bounds it, fp16 D = 128 (figures here and below: Hq / Hkv behind the tokens): from about 32 rows of a kv head on the matrix cores
+// beside the exponentials (16 x 4096 tokens, 16 / 8: 1145 us = 960 TFLOP/s, 2048 tokens at 129024 keys, 16 / 8: 1940 us =
+// 1125 TFLOP/s, where a large library product reaches 1144); below that the stream of keys (4 tokens each of 32 sequences of up to
+// 8192 keys, 32 / 8: 537 MB read in 97 us = 5.5 TB/s, with the merge 110 to 128 us, box to box) and, where there are few keys
+// too, the plan, the merge and the two launches (about 5 us).
 //
 // fp32 statistics throughout.  fp16: probabilities are rounded to fp16 for the second product (2^-11 of their value at
 // most; see softmax()), numerator and denominator from the same rounded values.  fp32: fp32 matrix instructions.
@@ -59,11 +60,12 @@ template <typename T, int D>
 struct Cfg {
   // Column tiles per wavefront, the fewest units of 128 keys of a piece, and the workgroups per CU that the cut aims at.
   // fp32 products take long enough for one column tile, and with half the rows in a tile and pieces of a single unit small
-  // batches spread over more workgroups (D = 64, against 2 tiles, 2 units, 2 workgroups): 3 ragged prompts of 200 tokens
-  // 16 us against 27, 16 decoding sequences at 2000 keys 25 against 31, 4096 tokens of one prompt 167 against 211.  A third
-  // workgroup fits there only (registers): 167 us against 225 with two; four pieces per CU: 300 tokens at 6000 keys 37 us
-  // against 32.  fp16 is slower with pieces of one unit (512 tokens of one prompt 25 us against 23) and gains nothing from
-  // three workgroups (D = 64: 4 x 1000 tokens 64 us against 62; D = 128 has registers for two).
+  // batches spread over more workgroups (D = 64, against 2 tiles, 2 units, 2 workgroups): 200 tokens of 3 prompts, 8 / 4,
+  // 16 us against 27, 16 decoding sequences at 2000 keys, 16 / 8, 25 against 31, 4096 tokens of one prompt, 8 / 4, 167 against
+  // 211.  A third workgroup fits there only (registers): 167 us against 225 with two; four pieces per CU: 300 tokens at 6000
+  // keys, 4 / 1, 37 us against 32.  fp16 is slower with pieces of one unit (512 tokens of one prompt, 32 / 8, D = 128, 25 us against
+  // 23) and gains nothing from three workgroups (D = 64: 4 x 1000 tokens at up to 2000 keys, 16 / 8, 64 us against 62; D = 128
+  // has registers for two).
   static constexpr int NT = D == 256 || sizeof(T) == 4 ? 1 : 2;
   static constexpr int MIN = sizeof(T) == 4 ? 1 : 2;
   static constexpr int AIM = D == 64 && sizeof(T) == 4 ? 3 : 2;
@@ -121,9 +123,9 @@ __device__ __forceinline__ int units_per_piece(const ChunkArgs &a, const Seq &fi
   return __builtin_amdgcn_readfirstlane(max(C::MIN, static_cast<int>(fminf(q, 1.0e9f))));
 }
 // Pieces of every tile of a sequence.  One that has few rows only streams keys, each its own: shorter pieces spread such
-// streams better over the device (32 sequences of 4000 keys 60 us, 65 us with whole pieces), while tiles of many rows that start
-// together share their keys in the caches.  Pieces that are short anyway stay whole (1 sequence of 32000 keys, pieces of 4 units
-// 35 us, of 2 units 38 us).
+// streams better over the device (32 sequences of up to 4000 keys, 16 / 8, 60 us, 65 us with whole pieces), while tiles of many
+// rows that start together share their keys in the caches.  Pieces that are short anyway stay whole (1 sequence of 32000 keys,
+// 16 / 8, pieces of 4 units 35 us, of 2 units 38 us).
 template <typename C>
 __device__ __forceinline__ int pieces_of(const Seq &s, int per) {
   const int p = C::kOwnBlocks && s.rows <= C::FEW && per >= 8 ? (per + 1) / 2 : per;
@@ -371,7 +373,7 @@ struct Wave {
   }
   // V^T fragments of a block, d tile by d tile.  fp32: product step (tk, e) takes keys tk * 16 + 4 g + e, g = 0 .. 3, so that
   // a lane's score register e is its right operand; d tile 4 h + i holds d = 64 h + 4 c + i, so that a lane's operands of four
-  // tiles are one 16-byte unit (single floats in their place: 3 x 819 tokens at 17600 keys, D = 128, 332 us against 298).
+  // tiles are one 16-byte unit (single floats in their place: 3 x 819 tokens at up to 17600 keys, 2 / 1, D = 128, 332 us against 298).
   __device__ __forceinline__ void read_v(int place, VFrag (&vf)[DT]) const {
     int va = vaddr + place;
     asm volatile("" : "+v"(va));
@@ -567,8 +569,8 @@ struct Wave {
     // multiplied, the next operands come from LDS, so a wavefront never waits for an LDS read that it has just made.  The
     // barrier that ends a stage stands in the middle of its last block, behind that block's last LDS read.
     // Of the two or three wavefronts of a SIMD the one at its products goes first: they fall out of step, and one's products run
-    // under another's exponentials (2048 tokens at 129024 keys 2130 -> 1995 us, 16 x 4096 tokens 1188 -> 1151 us).
-    if constexpr (!kHalf || D <= 128) {  // (fp32, D = 128: 4 x 512 tokens 80 us, 82 us without)
+    // under another's exponentials (2048 tokens at 129024 keys, 16 / 8, 2130 -> 1995 us, 16 x 4096 tokens 1188 -> 1151 us).
+    if constexpr (!kHalf || D <= 128) {  // (fp32, D = 128: 4 x 512 tokens, 16 / 8, 80 us, 82 us without; fp16, D = 256: spills)
       const int seen = position(0) + 1 - k0;  // keys of the piece that all rows see
       const int n_fast = few || seen <= 0 ? 0 : min(seen / KS, n_stages);
       if (n_fast > 0) {
@@ -873,7 +875,7 @@ struct Wave {
   }
   // Infinities and NaN of V as every row that sees their key has them, whatever it weighs: those that were cleaned away are added, and
   // a NaN that comes from a weight that rounds to 0 becomes the infinity.  Rare, so through memory and without a thought for speed.
-  // (Looking for such a NaN at the end of every piece: 16 x 4096 tokens of 16 heads of 128 in fp16 1142 -> 1150 us.)
+  // (Looking for such a NaN at the end of every piece: 16 x 4096 tokens, 16 / 8, 1142 -> 1150 us.)
   __device__ __forceinline__ void finish(int64_t part) {
     lds_barrier();
     const bool cleaned = flags[0] != 0, odd = flags[1] != 0;
@@ -935,7 +937,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
 
 // Adds the pieces of a cut tile: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  A workgroup takes up to 16 rows of the tile;
 // where these are fewer, or the pieces many, several threads share an element and take every P-th piece each, and their sums
-// are added up in a fixed tree through LDS (one row of 63 pieces: 5.6 us, 8.4 us one after the other).  A thread has four pieces
+// are added up in a fixed tree through LDS (one token of 63 pieces, 16 / 1: 5.6 us, 8.4 us one after the other).  A thread has four pieces
 // on their way at a time, and what bounds this kernel is the chain of such trips.
 constexpr int kMergeRows = 16;
 struct Sum {
@@ -966,38 +968,38 @@ __global__ __launch_bounds__(kMergeThreads) void chunk_merge_kernel(ChunkArgs a)
   while ((1 << log_rows) < rows) ++log_rows;
   const int items = (D / 4) << log_rows, parts = max(1, kMergeThreads / items);
   for (int at0 = 0; at0 < items; at0 += kMergeThreads) {  // (more than one pass only where parts is 1)
-  const int item = (at0 + tid) % items, part = tid / items, r = first + item / (D / 4), d = item % (D / 4) * 4;
-  const bool live = r < first + rows;
-  Sum sum{kMasked, 0.f, float4_t{0.f, 0.f, 0.f, 0.f}};
-  if (live) {
-    const int64_t base = (static_cast<int64_t>(pc.slot) * a.Hkv + hk) * a.slot_rows + r;
-    for (int s0 = part; s0 < pc.pieces; s0 += kAhead * parts) {
-      Sum got[kAhead];
+    const int item = (at0 + tid) % items, part = tid / items, r = first + item / (D / 4), d = item % (D / 4) * 4;
+    const bool live = r < first + rows;
+    Sum sum{kMasked, 0.f, float4_t{0.f, 0.f, 0.f, 0.f}};
+    if (live) {
+      const int64_t base = (static_cast<int64_t>(pc.slot) * a.Hkv + hk) * a.slot_rows + r;
+      for (int s0 = part; s0 < pc.pieces; s0 += kAhead * parts) {
+        Sum got[kAhead];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int64_t at = base + min(s0 + i * parts, pc.pieces - 1) * step;
-        got[i].m = a.part_ml[at * 2];
-        got[i].l = a.part_ml[at * 2 + 1];
-        got[i].o = *reinterpret_cast<const float4_t *>(a.part_o + at * D + d);
+        for (int i = 0; i < kAhead; ++i) {
+          const int64_t at = base + min(s0 + i * parts, pc.pieces - 1) * step;
+          got[i].m = a.part_ml[at * 2];
+          got[i].l = a.part_ml[at * 2 + 1];
+          got[i].o = *reinterpret_cast<const float4_t *>(a.part_o + at * D + d);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+          if (s0 + i * parts < pc.pieces) add_sum(sum, got[i]);
       }
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i)
-        if (s0 + i * parts < pc.pieces) add_sum(sum, got[i]);
     }
-  }
-  // (parts is a power of two, like all the sizes it is made from; one that had no piece adds nothing)
-  __shared__ Sum sums[kMergeThreads];
-  for (int half = parts / 2; half > 0; half /= 2) {
-    if (part >= half && part < 2 * half) sums[tid] = sum;
-    __syncthreads();
-    if (part < half) add_sum(sum, sums[tid + half * items]);
-  }
-  if (part > 0 || !live) continue;
-  const float inv = sum.l > 0.f ? 1.0f / sum.l : (sum.l == 0.f ? 0.f : sum.l);
-  const int rr = row0 + r, i = rr / a.group;
-  T *out = static_cast<T *>(a.out) + (static_cast<int64_t>(pc.c0 + i) * a.Hq + hk * a.group + (rr - i * a.group)) * D + d;
+    // (parts is a power of two, like all the sizes it is made from; one that had no piece adds nothing)
+    __shared__ Sum sums[kMergeThreads];
+    for (int half = parts / 2; half > 0; half /= 2) {
+      if (part >= half && part < 2 * half) sums[tid] = sum;
+      __syncthreads();
+      if (part < half) add_sum(sum, sums[tid + half * items]);
+    }
+    if (part > 0 || !live) continue;
+    const float inv = sum.l > 0.f ? 1.0f / sum.l : (sum.l == 0.f ? 0.f : sum.l);
+    const int rr = row0 + r, i = rr / a.group;
+    T *out = static_cast<T *>(a.out) + (static_cast<int64_t>(pc.c0 + i) * a.Hq + hk * a.group + (rr - i * a.group)) * D + d;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) stf(out + e, sum.o[e] * inv);
+    for (int e = 0; e < 4; ++e) stf(out + e, sum.o[e] * inv);
   }
 }
 
@@ -1053,11 +1055,11 @@ int launch(ChunkArgs a, const Sizes &z, hipStream_t st) {
   if (rc != AXHIP_OK) return rc;
   hipLaunchKernelGGL((chunk_attn_kernel<T, D>), dim3(static_cast<unsigned>(z.grid * a.Hkv)), dim3(kThreads), C::kLdsBytes, st, a);
   if (z.cut_tiles > 0) {
-    // 1024 threads where every tile has few rows or there are few tiles (1 row of 32768 keys: 40 us against 51), 256 where most
-    // workgroups find sixteen rows of few pieces or none (8 x 2000 rows: 109 us against 123).  Fewer rows a workgroup, and
-    // more threads an element, as long as that leaves a workgroup per CU (16 heads of one token over 128000 keys 31 us, 120 us
-    // with 16 rows; 64 tokens at 16000 keys 33 us against 61), of 256 threads four (512 tokens at 8000 keys 60 us against 63;
-    // 8 x 2000 tokens 205 us with 8 rows, 200 us with 16).
+    // 1024 threads where every tile has few rows or there are few tiles (1 token of 128000 keys, 16 / 1: 31 us, 41 us with 256), 256
+    // where most workgroups find sixteen rows of few pieces or none (8 x 2000 tokens, 16 / 8: 195 us, 208 us with 1024).
+    // Fewer rows a workgroup, and more threads an element, as long as that leaves a workgroup per CU (of 256 threads four): with 16
+    // rows the 1 token of 128000 keys takes 123 us, 64 tokens at 16000 keys, 16 / 8, 38 us instead of 30, 512 tokens at
+    // 8000 keys, 16 / 8, 55 instead of 54.
     const int cus = device_cu_count(), tiles = static_cast<int>(z.cut_tiles * a.Hkv);
     const auto groups = [&](int rows) { return (z.slot_rows + rows - 1) / rows; };
     const bool wide = groups(kMergeRows) == 1 || tiles * groups(kMergeRows) <= cus;

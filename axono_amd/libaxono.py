@@ -949,7 +949,7 @@ def rotary_inv_freq(rotary_dim: int, theta: float = 10000.0, kind: str = "plain"
     """The frequency table of rotary_qk / rotary_append_paged, FLOAT32 (rotary_dim / 2,) on `device`, and the factor on
     cosine and sine that belongs to it: theta^(-2i / rotary_dim) as it is ("plain"), divided by `factor` ("linear"), with
     theta raised ("ntk"), or with the slow frequencies divided and the fast ones kept ("yarn": between slow_turns and
-    fast_turns turns over trained_len positions)."""
+    fast_turns turns over trained_len positions, linearly in the turns).  rotary_qk takes any other FLOAT32 table as well."""
     op = "rotary_inv_freq"
     if kind not in ROTARY_KINDS:
         raise ValueError(f"rotary_inv_freq: kind must be one of {sorted(ROTARY_KINDS)}, got {kind!r}")

@@ -395,7 +395,7 @@ AXHIP_API int axhip_rope_with_cos_sin(const void *x, const float *cos_t, const f
  *   q [rows, q_heads, dim], k [rows, k_heads, dim], `dtype`; rows q_stride / k_stride elements apart, heads contiguous
  *   pos device int64[rows]; inv_freq device fp32[rotary_dim / 2] (axhip_rotary_inv_freq); scale: on cosine and sine
  *   q_out, k_out contiguous; each may be its input when that is contiguous (else AXHIP_INVALID_ARGUMENT)
- * q_heads or k_heads may be 0.  dim % 8 == 0, dim <= 512, rotary_dim even.  Interleaved pairs start on even elements:
+ * q_heads or k_heads may be 0.  dim % 8 == 0, dim <= 512, rotary_dim even; rows < 2^31, at most 65535 heads.  Interleaved pairs start on even elements:
  * pointers and strides that would put one across a boundary of two elements return AXHIP_INVALID_ARGUMENT.
  * The reference rotates whole heads in the half layout only (ops::cuda::Rope, src/ops/cuda/sequence.cu:84-101,318-342). */
 AXHIP_API int axhip_rotary_qk(const void *q, int64_t q_stride, const void *k, int64_t k_stride, const int64_t *pos,
@@ -404,10 +404,12 @@ AXHIP_API int axhip_rotary_qk(const void *q, int64_t q_stride, const void *k, in
                               axhip_stream stream);
 
 /* The table for axhip_rotary_qk, computed on the host into host memory (upload it once): f_i = theta^(-2 i / rotary_dim),
- *   LINEAR  f_i / factor;   NTK  theta replaced by theta factor^(rotary_dim / (rotary_dim - 2));
+ *   LINEAR  f_i / factor;   NTK  theta replaced by theta factor^(rotary_dim / (rotary_dim - 2)) (one pair: as it is);
  *   YARN    f_i k + (f_i / factor)(1 - k), k = clamp((trained_len f_i / 2 pi - slow_turns) / (fast_turns - slow_turns), 0, 1):
  *           pairs that turn at least fast_turns times over the trained context keep their frequency, pairs that turn
- *           at most slow_turns times are divided.  *scale = 0.1 ln(factor) + 1 for factor > 1.
+ *           at most slow_turns times are divided, linearly in the turns between them (not in the pair's number, as some
+ *           loaders of checkpoints have it).  *scale = 0.1 ln(factor) + 1 for factor > 1.
+ * Any other table (bands of wavelengths, a factor for each pair) can be made by the caller: the operators take what inv_freq holds.
  * theta > 0, factor > 0 (PLAIN ignores it), rotary_dim even and at most 512; trained_len, fast_turns and slow_turns are
  * read for YARN only.  *scale (may be NULL) is 1 for the other kinds.  No reference counterpart. */
 #define AXHIP_ROTARY_PLAIN 0
@@ -433,8 +435,8 @@ AXHIP_API int axhip_rotary_inv_freq(int kind, double theta, int rotary_dim, doub
  * pos: int64 [tokens] (pos_axes 1), int64 [3, tokens] (pos_axes 3: pair i turns by axis 1 if i % 3 == 1 and
  * i < 3 h_sec, by axis 2 if i % 3 == 2 and i < 3 w_sec, else by axis 0), or NULL: the key position.
  * A position outside the table and a page number outside [0, n_pages) skip the k and v rows; q is written all the same.
- * D % 8 == 0, D <= 512, pools 16-byte aligned, B <= 2^20; q_out apart from q, k and v.  Equals rms_norm, rotation, cast and axhip_kv_append_paged in that order;
- * the reference runs them one by one over a cache that it copies (examples/vlm/qwen3vl/model.py:353-364). */
+ * D % 8 == 0, D <= 512, Hq <= 32767, Hkv <= 16383, pools 16-byte aligned, B <= 2^20; q_out apart from q, k and v.  Equals
+ * rms_norm, rotation, cast and axhip_kv_append_paged in that order; the reference runs them one by one over a cache that it copies (examples/vlm/qwen3vl/model.py:353-364). */
 AXHIP_API int axhip_rotary_append_paged(const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v,
                                         int64_t v_stride, int dtype, const void *q_weight, const void *k_weight,
                                         int w_dtype, float eps, int norm, const int64_t *pos, int pos_axes,
@@ -447,9 +449,10 @@ AXHIP_API int axhip_rotary_append_paged(const void *q, int64_t q_stride, const v
 /* Causal attention of the new tokens over the cache that already holds their keys and values:
  *   out_i = softmax(q_i . K[0 .. p]^T / sqrt(D)) V[0 .. p],  p = min(start[b] + i, max_len - 1); p < 0: zeros.
  * From one token a sequence (decode) over drafts of a few to chunks of a prompt, mixed in one launch.
- *   q, out [tokens, Hq, D] of `dtype` (FLOAT16 or FLOAT32), the pools' type; D 64, 128 or 256; Hq % Hkv == 0
+ *   q, out [tokens, Hq, D] of `dtype` (FLOAT16 or FLOAT32), the pools' type; D 64, 128 or 256; Hq % Hkv == 0; q, out and
+ *   pools 16-byte aligned
  *   max_q bounds every sequence's new tokens (more are not computed), max_len every p + 1; max_pages * 128 >= max_len;
- *   tokens * Hq <= 2^30, B <= 2^20, Hkv <= 1024, and B * Hkv small enough for a launch (under 2^24 workgroups)
+ *   max_len <= 2^30, tokens * Hq <= 2^30, B <= 2^20, Hkv <= 1024, and B * Hkv small enough for a launch (under 2^24 workgroups)
  *   workspace: axhip_chunk_attention_paged_workspace_bytes(...) bytes, 16-byte aligned, contents free; launches
  *   that may overlap in time need one each (captured graphs that replay side by side too)
  * Page numbers outside [0, n_pages) are clamped into the pool: wrong values, never an access outside it.  Infinities and
@@ -534,7 +537,7 @@ AXHIP_API int axhip_argmax(const void *x, int64_t *out, int dtype, int64_t rows,
  *   repetition, presence, frequency  device fp32 [rows] or NULL (1, 0, 0)
  *   bias_ids, bias  device int32 / fp32 [rows, bias_count <= 16384], ids outside the vocabulary are padding
  *   allowed      device uint32 bits, token v of a row: bit v % 32 of word v / 32; rows allowed_stride words apart; or NULL
- * At most 65535 rows.  Ids outside the vocabulary are passed over.  The order of the history does not change a bit of the result.
+ * At most 65535 rows, vocab <= 2^30, max_history < 2^30.  Ids outside the vocabulary are passed over.  The order of the history does not change a bit of the result.
  * No reference counterpart (its example picks the plain argmax, examples/vlm/qwen3vl/model.py:846-858). */
 AXHIP_API int axhip_logits_process(const void *logits, int64_t logits_stride, int dtype, const void *history,
                                    int history_dtype, int64_t history_row_stride, int64_t history_token_stride,
