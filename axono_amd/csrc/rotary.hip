@@ -354,7 +354,7 @@ AXHIP_API int axhip_rotary_inv_freq(int kind, double theta, int rotary_dim, doub
                                     double fast_turns, double slow_turns, float *inv_freq, float *scale) {
   if (kind < AXHIP_ROTARY_PLAIN || kind > AXHIP_ROTARY_YARN || rotary_dim <= 0 || rotary_dim % 2 != 0 || rotary_dim > 2 * kMaxPairs)
     return AXHIP_INVALID_ARGUMENT;
-  if (!(theta > 0.0) || !(factor > 0.0)) return AXHIP_INVALID_ARGUMENT;
+  if (!(theta > 0.0) || (kind != AXHIP_ROTARY_PLAIN && !(factor > 0.0))) return AXHIP_INVALID_ARGUMENT;
   if (kind == AXHIP_ROTARY_YARN && (trained_len <= 0 || !(fast_turns > slow_turns))) return AXHIP_INVALID_ARGUMENT;
   if (!inv_freq) return AXHIP_INVALID_PTR;
   const double two_pi = 6.283185307179586477;

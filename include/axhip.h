@@ -395,8 +395,9 @@ AXHIP_API int axhip_rope_with_cos_sin(const void *x, const float *cos_t, const f
  *   q [rows, q_heads, dim], k [rows, k_heads, dim], `dtype`; rows q_stride / k_stride elements apart, heads contiguous
  *   pos device int64[rows]; inv_freq device fp32[rotary_dim / 2] (axhip_rotary_inv_freq); scale: on cosine and sine
  *   q_out, k_out contiguous; each may be its input when that is contiguous (else AXHIP_INVALID_ARGUMENT)
- * q_heads or k_heads may be 0.  dim % 8 == 0, dim <= 512, rotary_dim even; rows < 2^31, at most 65535 heads.  Interleaved pairs start on even elements:
- * pointers and strides that would put one across a boundary of two elements return AXHIP_INVALID_ARGUMENT.
+ * q_heads or k_heads may be 0.  dim % 8 == 0, dim <= 512, rotary_dim even; rows < 2^31, at most 65535 heads.
+ * Interleaved pairs start on even elements: pointers and strides that would put one across a boundary of two elements
+ * return AXHIP_INVALID_ARGUMENT.
  * The reference rotates whole heads in the half layout only (ops::cuda::Rope, src/ops/cuda/sequence.cu:84-101,318-342). */
 AXHIP_API int axhip_rotary_qk(const void *q, int64_t q_stride, const void *k, int64_t k_stride, const int64_t *pos,
                               const float *inv_freq, float scale, int interleaved, int rotary_dim, void *q_out,
@@ -436,7 +437,8 @@ AXHIP_API int axhip_rotary_inv_freq(int kind, double theta, int rotary_dim, doub
  * i < 3 h_sec, by axis 2 if i % 3 == 2 and i < 3 w_sec, else by axis 0), or NULL: the key position.
  * A position outside the table and a page number outside [0, n_pages) skip the k and v rows; q is written all the same.
  * D % 8 == 0, D <= 512, Hq <= 32767, Hkv <= 16383, pools 16-byte aligned, B <= 2^20; q_out apart from q, k and v.  Equals
- * rms_norm, rotation, cast and axhip_kv_append_paged in that order; the reference runs them one by one over a cache that it copies (examples/vlm/qwen3vl/model.py:353-364). */
+ * rms_norm, rotation, cast and axhip_kv_append_paged in that order; the reference runs them one by one over a cache that
+ * it copies (examples/vlm/qwen3vl/model.py:353-364). */
 AXHIP_API int axhip_rotary_append_paged(const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v,
                                         int64_t v_stride, int dtype, const void *q_weight, const void *k_weight,
                                         int w_dtype, float eps, int norm, const int64_t *pos, int pos_axes,
@@ -537,7 +539,8 @@ AXHIP_API int axhip_argmax(const void *x, int64_t *out, int dtype, int64_t rows,
  *   repetition, presence, frequency  device fp32 [rows] or NULL (1, 0, 0)
  *   bias_ids, bias  device int32 / fp32 [rows, bias_count <= 16384], ids outside the vocabulary are padding
  *   allowed      device uint32 bits, token v of a row: bit v % 32 of word v / 32; rows allowed_stride words apart; or NULL
- * At most 65535 rows, vocab <= 2^30, max_history < 2^30.  Ids outside the vocabulary are passed over.  The order of the history does not change a bit of the result.
+ * At most 65535 rows, vocab <= 2^30, max_history < 2^30.  Ids outside the vocabulary are passed over.  The order of the history
+ * does not change a bit of the result.
  * No reference counterpart (its example picks the plain argmax, examples/vlm/qwen3vl/model.py:846-858). */
 AXHIP_API int axhip_logits_process(const void *logits, int64_t logits_stride, int dtype, const void *history,
                                    int history_dtype, int64_t history_row_stride, int64_t history_token_stride,

@@ -172,3 +172,13 @@ def test_sizes_that_no_launch_takes_are_refused():
     assert append(B=(1 << 20) + 1) == INVALID
     assert chunk(T=1 << 20, B=1 << 20, hq=32, hk=32) == INVALID          # 2^25 workgroups
     assert logits(rows=1, bc=16385) == INVALID
+
+
+def test_a_plain_frequency_table_looks_at_theta_alone():
+    """the factor and the turns of the other kinds are not read"""
+    want = inv_freq(0, 1e4, 64)
+    for rest in ((0.0,), (-3.0, -1, 1.0, 2.0), (float("nan"), 0, float("nan"), float("nan"))):
+        rc, f, s = inv_freq(0, 1e4, 64, *rest)
+        assert (rc, s) == (OK, 1.0)
+        np.testing.assert_array_equal(f, want[1])
+    assert inv_freq(1, 1e4, 64, 2.0, -1, 0.0, 0.0)[0] == OK and inv_freq(2, 1e4, 64, 2.0, -1, 0.0, 0.0)[0] == OK
