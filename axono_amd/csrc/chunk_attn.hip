@@ -937,7 +937,7 @@ __global__ __launch_bounds__(kThreads, (Cfg<T, D>::kLdsBytes <= 80 * 1024 ? 2 : 
 
 // Adds the pieces of a cut tile: out = sum_s o_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  A workgroup takes up to 16 rows of the tile;
 // where these are fewer, or the pieces many, several threads share an element and take every P-th piece each, and their sums
-// are added up in a fixed tree through LDS (one token of 63 pieces, 16 / 1: 5.6 us, 8.4 us one after the other).  A thread has four pieces
+// are added up in a fixed tree through LDS (one token of 63 pieces, 16 / 8: 5.6 us, 8.4 us one after the other).  A thread has four pieces
 // on their way at a time, and what bounds this kernel is the chain of such trips.
 constexpr int kMergeRows = 16;
 struct Sum {
