@@ -49,7 +49,7 @@ struct ChunkArgs {
   const int32_t *page_table, *cu, *start;
   void *out;
   float *part_o;   // [slots][slot_rows][D]
-  float *part_ml;  // [slots][slot_rows][2]: maximum (log2 units), sum
+  float *part_ml;  // [slots][slot_rows][2]: level (log2 units), sum
   int tokens, B, Hq, Hkv, group, max_q, max_len, max_pages, n_pages;
   int slots, slot_rows, target;  // target: pieces the launch aims at
   int merge_rows;                // rows per workgroup of the merge
@@ -434,7 +434,8 @@ struct Wave {
   // fp16: the level lies 2^kBelow under the maximum that set it, so that p is 2^10 at the maximum and 2^15 at most: below
   // 2^-24 of the largest weight of a row its others lose bits, below 2^-35 they are lost.  (Against the maximum itself those
   // under 2^-25 would be, and 65536 such keys hold 2^-9 of the sum.)
-  static constexpr float kBelow = kHalf ? 10.f : 0.f, kTop = kHalf ? 32768.f : 256.f;
+  // fp32: the level lies 2^8 above, so that p is at most 1 and a sum of weighted values ends where the sum of the values does.
+  static constexpr float kBelow = kHalf ? 10.f : -8.f, kTop = kHalf ? 32768.f : 1.f;
   // Large scores: the level is a product rounded to fp32, taken a step or two low so that the largest score never lies under what it
   // was meant to be over.  Where a step is more than kTop leaves room for (levels past 2^23) p ends at kTop: scores within
   // 2^-22 of the largest then weigh the same, which is what the rounding of their own sums leaves of them.

@@ -200,3 +200,36 @@ def test_captured_calls_follow_what_is_cut(dtype):
             assert ps.picking_error(got, *ps.picking_want(q, k, v, table, n, start)) <= 0.25, (n, start)
             eager = L.chunk_attention_paged(*at, T, longest)
             np.testing.assert_array_equal(eager.numpy()[:len(q)].view(np.uint8), got.view(np.uint8))
+
+
+@pytest.mark.parametrize("heads", [(4, 2, 64), (2, 1, 128), (2, 2, 256)])
+@pytest.mark.parametrize("batch", [([1], [41]), ([6], [300]), ([150], [100]), ([3], [9000])])
+def test_finite_values_near_the_end_of_fp32(heads, batch):
+    """a row's weighted mean of values up to 3e35 .. 1e37 is finite wherever the sum of weights of at most 1 times them is: 3.4e38 over
+    the number of keys.  Scores rise by 5 on the way, so that what is summed first was the largest then."""
+    (n, start), (hq, hk, d) = batch, heads
+    rng = np.random.default_rng(1)
+    table, n_pages = ps.pages_for(n, start, rng)
+    keys = start[0] + n[0]
+    q, k = np.zeros((n[0], hq, d), np.float32), np.zeros((n_pages, hk, 128, d), np.float32)
+    q[..., 0] = 8
+    for key in range(keys):                     # in steps of a fifth of what the first token sees
+        k[table[0, key // 128], :, key % 128, 0] = np.sqrt(d) / 8 * min(5 * key // (start[0] + 1), 5)
+    v = (rng.uniform(0.5, 1, k.shape) * 3.4e38 / keys * 0.9).astype(np.float32)
+    got = ps.chunk(q, k, v, table, ps.cu_of(n), start, n[0], keys)
+    want, tol = ps.chunk_want(q, k, v, table, n, start, keys)
+    assert np.isfinite(want).all()
+    ps.assert_within(got, want, tol)
+
+
+@pytest.mark.parametrize("batch", [([1], [41]), ([150], [100]), ([3], [9000])])
+def test_finite_values_near_nothing(batch):
+    """values of 1e-37: a weight of 2^-8 makes a product denormal, off by 2^-150, the mean by 2^-142 (and its own rounding)"""
+    n, start = batch
+    rng = np.random.default_rng(2)
+    table, n_pages = ps.pages_for(n, start, rng)
+    q, k = np.zeros((n[0], 4, 64), np.float32), np.zeros((n_pages, 2, 128, 64), np.float32)
+    v = rng.uniform(0.5e-37, 1e-37, k.shape).astype(np.float32)
+    got = ps.chunk(q, k, v, table, ps.cu_of(n), start, n[0], start[0] + n[0])
+    want, tol = ps.chunk_want(q, k, v, table, n, start, start[0] + n[0])
+    ps.assert_within(got, want, tol + 2.0 ** -141)
