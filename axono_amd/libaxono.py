@@ -1064,13 +1064,16 @@ def chunk_attention_paged(q: Tensor, k_pool: Tensor, v_pool: Tensor, page_table:
     n_pages, hkv, _, dk = k_pool.shape
     if dk != d or hkv == 0 or hq % hkv != 0:
         raise AxhipError(op, Status.SHAPE_MISMATCH)
+    max_q, max_len = int(max_q), int(max_len)
+    if max_q < 0 or not 0 <= max_len <= min(page_table.shape[1] * PAGE_KEYS, 1 << 30):
+        raise AxhipError(op, Status.INVALID_ARGUMENT)
     if out is None:
         out = _new(q.dtype, [tokens, hq, d], q)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise AxhipError(op, Status.SHAPE_MISMATCH)
     _use_device(op, q)
     lib = _lib_()
-    sizes = (int(q.dtype), tokens, B, hq, hkv, d, int(max_q), int(max_len))
+    sizes = (int(q.dtype), tokens, B, hq, hkv, d, min(max_q, tokens), max_len)
     need = lib.axhip_chunk_attention_paged_workspace_bytes(*sizes)
     ws = workspace if workspace is not None else _workspace(need, q)
     check(lib.axhip_chunk_attention_paged(q.data_ptr, k_pool.data_ptr, v_pool.data_ptr, page_table.data_ptr, cu_tokens.data_ptr,

@@ -253,3 +253,17 @@ def test_pages_beyond_four_gigabytes():
         for i, p in enumerate(where):
             L.copy_bytes(back, i * page_bytes, large, p * page_bytes, page_bytes)
         np.testing.assert_array_equal(back.to_numpy(), small.to_numpy())
+
+
+def test_bounds_wider_than_an_int_do_not_wrap():
+    """max_q of 2^32 bounds nothing; a max_len that the page table does not hold is refused, whatever its low bits say"""
+    n, start = [3, 1], [200, 5]
+    q, k, v, table = ps.picking(n, start, 4, 2, 64, np.float16)
+    args = [hip(a) for a in (q, k, v, table, ps.cu_of(n), np.array(start, np.int32))]
+    want = L.chunk_attention_paged(*args, 3, 203).numpy()
+    for max_q in (1 << 32, (1 << 40) + 1, 1 << 31):
+        out = hip(np.full(q.shape, 9, np.float16))
+        np.testing.assert_array_equal(L.chunk_attention_paged(*args, max_q, 203, out=out).numpy(), want)
+    for bad in ((3, 1 << 32), (3, (1 << 32) + 203), (3, -1), (-1, 203), (-(1 << 32), 203)):
+        with pytest.raises(AxhipError):
+            L.chunk_attention_paged(*args, *bad)
